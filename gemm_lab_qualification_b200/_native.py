@@ -27,6 +27,8 @@ STATUS_NAMES = ("ok", "invalid_argument", "shape", "split", "workspace", "output
 MAX_SPLIT = 8
 MAX_RANKS = 8
 STATIC_GATHER_SLOTS = 64
+# enum glq_activation, by the names the operators take
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
 FLAG_NO_PDL = 1 << 0
 FLAG_STATIC_WEIGHTS = 1 << 1
 
@@ -54,6 +56,28 @@ SIGNATURES = {
     "glq_linear_workspace_bytes": (ctypes.c_size_t, [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I64]),
     "glq_plan": (_INT, [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I64, _I64, _INT, _INT,
                         _PINT, _PINT]),
+    "glq_fused_linear": (_INT, [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _INT, _VP, _I64, _VP, _I64, _VP, _I64,
+                                _I64, _I64, _I64, _VP, ctypes.c_size_t, _VP, ctypes.c_uint]),
+    "glq_fused_linear_workspace_bytes": (ctypes.c_size_t, [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I64]),
+    "glq_fused_linear_backward": (_INT, [_INT, _VP, _I64, _VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _INT, _VP,
+                                         _I64, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _VP, ctypes.c_size_t, _VP,
+                                         ctypes.c_uint]),
+    "glq_fused_linear_backward_workspace_bytes": (ctypes.c_size_t, [_INT, _VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64,
+                                                                    _INT, _INT, _I64, _I64, _I64]),
+    "glq_gated_linear": (_INT, [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _VP, _INT, _VP, _VP,
+                                _I64, _VP, _I64, _I64, _I64, _I64, _VP, ctypes.c_size_t, _VP, ctypes.c_uint]),
+    "glq_gated_linear_workspace_bytes": (ctypes.c_size_t, [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I64, _I64,
+                                                           _I64, _I64, _I64]),
+    "glq_gated_linear_backward": (_INT, [_INT, _VP, _I64, _VP, _VP, _I64, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I64,
+                                         _I64, _INT, _VP, _I64, _VP, _VP, _I64, _I64, _VP, _VP, _I64, _I64, _I64, _VP,
+                                         ctypes.c_size_t, _VP, ctypes.c_uint]),
+    "glq_gated_linear_backward_workspace_bytes": (ctypes.c_size_t, [_INT, _VP, _I64, _I64, _VP, _I64, _I64, _VP, _I64,
+                                                                    _I64, _INT, _I64, _I64, _I64]),
+    "glq_layer_norm": (_INT, [_INT, _VP, _I64, _VP, _VP, ctypes.c_double, _VP, _I64, _VP, _VP, _I64, _I64, _VP,
+                              ctypes.c_uint]),
+    "glq_layer_norm_backward": (_INT, [_INT, _VP, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _I64, _VP, _VP, _I64, _I64,
+                                       _VP, ctypes.c_size_t, _VP, ctypes.c_uint]),
+    "glq_layer_norm_backward_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
     "glq_path_name": (ctypes.c_char_p, [_INT]),
     "glq_status_string": (ctypes.c_char_p, [_INT]),
     "glq_device_error": (_INT, [ctypes.POINTER(ctypes.c_uint), _INT]),

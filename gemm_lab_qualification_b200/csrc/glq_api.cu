@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <mutex>
 
+#include "glq_ffn.h"
 #include "glq_internal.h"
 
 namespace glq {
@@ -55,7 +56,8 @@ int device_state(DeviceState** out) {
     st.sm_count = sms > 0 ? sms : 148;
     void* word = nullptr;
     if (cudaGetSymbolAddress(&word, g_device_error_word) != cudaSuccess ||
-        tc_prepare_device() != cudaSuccess || gemv_prepare_device() != cudaSuccess) {
+        tc_prepare_device() != cudaSuccess || gemv_prepare_device() != cudaSuccess ||
+        pair_prepare_device() != cudaSuccess || skinny_prepare_device() != cudaSuccess) {
       cudaGetLastError();
       st.status = GLQ_ERR_CUDA;
       return;
@@ -129,6 +131,15 @@ int static_gather_scratch(unsigned int** out) {
 }
 
 }  // namespace
+
+int current_device(int* sm_count, unsigned int** error_word) {
+  DeviceState* st = nullptr;
+  const int v = device_state(&st);
+  if (v != GLQ_OK) return v;
+  *sm_count = st->sm_count;
+  *error_word = st->error_word;
+  return GLQ_OK;
+}
 
 OperandLayout classify(const Problem& p) {
   constexpr int64_t esz = 2;

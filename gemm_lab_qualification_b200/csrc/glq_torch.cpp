@@ -9,6 +9,7 @@
 // contiguity rule) and the launch in one native call on torch's current
 // stream.  Library failures come back as the glq_status so that Python raises
 // the same GlqError as the ctypes binding.
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -129,6 +130,270 @@ std::tuple<int, int, int> linear_gather(const at::Tensor& a, const at::Tensor& b
   return {status, path, split};
 }
 
+// ---------------------------------------------------------------- feed-forward operators
+//
+// Each allocates its outputs and workspace from torch's caching allocator on
+// the current stream of the operands' device (made current for the call) and
+// returns (glq_status, outputs...).
+
+using OptTensor = c10::optional<at::Tensor>;
+
+int dtype_of(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? GLQ_DTYPE_F16 : GLQ_DTYPE_BF16; }
+
+cudaStream_t stream_of(const at::Tensor& t) {
+  return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
+}
+
+void check_vector(const OptTensor& v, const at::Tensor& a, int64_t n, const char* name) {
+  if (!v.has_value()) return;
+  if (v->dim() != 1 || v->size(0) != n || v->device() != a.device() || v->scalar_type() != a.scalar_type()) {
+    throw py::value_error(std::string(name) + " tensor has the wrong shape, device, or dtype");
+  }
+  if (n > 1 && v->stride(0) != 1) throw py::value_error(std::string(name) + " tensor must be contiguous");
+}
+
+void check_matrix(const at::Tensor& t, const at::Tensor& a, int64_t m, int64_t n, const char* name) {
+  if (t.dim() != 2 || t.size(0) != m || t.size(1) != n || t.device() != a.device() ||
+      t.scalar_type() != a.scalar_type()) {
+    throw py::value_error(std::string(name) + " tensor has the wrong shape, device, or dtype");
+  }
+}
+
+// An input read by rows: itself if its columns are contiguous and its rows
+// do not overlap, else a contiguous copy.
+at::Tensor by_rows(const at::Tensor& t) {
+  const bool rows = (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+  return rows ? t : t.contiguous();
+}
+
+void* ptr(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+// A workspace of `bytes`; keep it alive until the launches are queued.
+struct Workspace {
+  at::Tensor t;
+  size_t bytes;
+  Workspace(size_t n, const at::Tensor& like) : bytes(n) {
+    if (n) t = at::empty({static_cast<int64_t>(n)}, like.options().dtype(at::kByte));
+  }
+  void* data() const { return bytes ? t.data_ptr() : nullptr; }
+};
+
+// Gradient of b [k, n] in b's own order: the transpose of [n, k] rows for a
+// weight's W.t(), else [k, n] rows.
+at::Tensor empty_like_weight(const at::Tensor& b) {
+  const int64_t k = b.size(0), n = b.size(1);
+  const bool nk = b.stride(0) == 1 && !(b.stride(1) == 1 && k > 1 && n > 1);
+  return nk ? at::empty({n, k}, b.options()).t() : at::empty({k, n}, b.options());
+}
+
+std::tuple<int, at::Tensor, OptTensor> fused_linear(const at::Tensor& a, const at::Tensor& b, const OptTensor& bias,
+                                                    int activation, const OptTensor& residual, const OptTensor& output,
+                                                    const OptTensor& preact, bool return_preact, int64_t flags) {
+  check_inputs(a, b, "fused_linear");
+  const c10::cuda::CUDAGuard guard(a.device());
+  const int64_t m = a.size(0), k = a.size(1), n = b.size(1);
+  check_vector(bias, a, n, "bias");
+  at::Tensor res;
+  if (residual.has_value()) {
+    check_matrix(*residual, a, m, n, "residual");
+    res = by_rows(*residual);
+  }
+  at::Tensor y = output.has_value() ? *output : at::empty({m, n}, a.options());
+  if (output.has_value()) check_output(y, a, m, n);
+  OptTensor z = preact;
+  if (z.has_value()) {
+    check_output(*z, a, m, n);
+  } else if (return_preact) {
+    z = at::empty({m, n}, a.options());
+  }
+  const Workspace ws(glq_fused_linear_workspace_bytes(dtype_of(a), a.data_ptr(), a.stride(0), a.stride(1), b.data_ptr(),
+                                                      b.stride(0), b.stride(1), m, n, k),
+                     a);
+  const int status = glq_fused_linear(
+      dtype_of(a), a.data_ptr(), a.stride(0), a.stride(1), b.data_ptr(), b.stride(0), b.stride(1), ptr(bias), activation,
+      res.defined() ? res.data_ptr() : nullptr, res.defined() ? res.stride(0) : 0, ptr(z), z.has_value() ? z->stride(0) : 0,
+      y.data_ptr(), y.stride(0), m, n, k, ws.data(), ws.bytes, stream_of(a), static_cast<unsigned int>(flags));
+  return {status, y, z};
+}
+
+std::tuple<int, OptTensor, OptTensor, OptTensor> fused_linear_backward(const at::Tensor& grad, const at::Tensor& a,
+                                                                       const at::Tensor& b, const OptTensor& preact,
+                                                                       int activation, bool want_a, bool want_b,
+                                                                       bool has_bias, int64_t flags) {
+  check_inputs(a, b, "fused_linear_backward");
+  const c10::cuda::CUDAGuard guard(a.device());
+  const int64_t m = a.size(0), k = a.size(1), n = b.size(1);
+  check_matrix(grad, a, m, n, "grad_output");
+  const at::Tensor dy = by_rows(grad);
+  at::Tensor z;
+  if (activation != GLQ_ACT_NONE) {
+    if (!preact.has_value()) throw py::value_error("the backward pass of an activation needs preact");
+    check_matrix(*preact, a, m, n, "preact");
+    z = by_rows(*preact);
+  }
+  OptTensor da, db, dbias;
+  if (want_a) da = at::empty({m, k}, a.options());
+  if (want_b) db = empty_like_weight(b);
+  if (has_bias) dbias = at::empty({n}, a.options());
+  const Workspace ws(glq_fused_linear_backward_workspace_bytes(dtype_of(a), dy.data_ptr(), dy.stride(0), a.data_ptr(),
+                                                               a.stride(0), a.stride(1), b.data_ptr(), b.stride(0),
+                                                               b.stride(1), activation, has_bias ? 1 : 0, m, n, k),
+                     a);
+  const int status = glq_fused_linear_backward(
+      dtype_of(a), dy.data_ptr(), dy.stride(0), z.defined() ? z.data_ptr() : nullptr, z.defined() ? z.stride(0) : 0,
+      a.data_ptr(), a.stride(0), a.stride(1), b.data_ptr(), b.stride(0), b.stride(1), activation,
+      ptr(da), da.has_value() ? da->stride(0) : 0, ptr(db),
+      db.has_value() ? db->stride(0) : 0, db.has_value() ? db->stride(1) : 0, ptr(dbias), m, n, k,
+      ws.data(), ws.bytes, stream_of(a), static_cast<unsigned int>(flags));
+  return {status, da, db, dbias};
+}
+
+void check_pair(const at::Tensor& a, const at::Tensor& b_gate, const at::Tensor& b_up, const std::string& op) {
+  check_inputs(a, b_gate, op);
+  check_inputs(a, b_up, op);
+  if (b_gate.size(1) != b_up.size(1)) {
+    throw py::value_error("incompatible dimensions: " + shape_str(b_gate) + " and " + shape_str(b_up));
+  }
+}
+
+std::tuple<int, at::Tensor, OptTensor, OptTensor> gated_linear(const at::Tensor& a, const at::Tensor& b_gate,
+                                                               const at::Tensor& b_up, const OptTensor& bias_gate,
+                                                               const OptTensor& bias_up, int activation,
+                                                               const OptTensor& output, const OptTensor& gate,
+                                                               const OptTensor& up, bool return_preact, int64_t flags) {
+  check_pair(a, b_gate, b_up, "gated_linear");
+  const c10::cuda::CUDAGuard guard(a.device());
+  const int64_t m = a.size(0), k = a.size(1), n = b_gate.size(1);
+  check_vector(bias_gate, a, n, "bias_gate");
+  check_vector(bias_up, a, n, "bias_up");
+  at::Tensor y = output.has_value() ? *output : at::empty({m, n}, a.options());
+  if (output.has_value()) check_output(y, a, m, n);
+  OptTensor g = gate, u = up;
+  if (g.has_value() != u.has_value()) throw py::value_error("gate and up are given together");
+  if (g.has_value()) {
+    check_output(*g, a, m, n);
+    check_output(*u, a, m, n);
+    if (m > 1 && g->stride(0) != u->stride(0)) throw py::value_error("gate and up need one row stride");
+  } else if (return_preact) {
+    g = at::empty({m, n}, a.options());
+    u = at::empty({m, n}, a.options());
+  }
+  const int dtype = dtype_of(a);
+  const Workspace ws(
+      glq_gated_linear_workspace_bytes(dtype, a.data_ptr(), a.stride(0), a.stride(1), b_gate.data_ptr(),
+                                       b_gate.stride(0), b_gate.stride(1), b_up.data_ptr(), b_up.stride(0),
+                                       b_up.stride(1), m, n, k),
+      a);
+  const int status = glq_gated_linear(
+      dtype, a.data_ptr(), a.stride(0), a.stride(1), b_gate.data_ptr(), b_gate.stride(0), b_gate.stride(1),
+      b_up.data_ptr(), b_up.stride(0), b_up.stride(1), ptr(bias_gate), ptr(bias_up), activation,
+      ptr(g), ptr(u), g.has_value() ? g->stride(0) : 0, y.data_ptr(), y.stride(0),
+      m, n, k, ws.data(), ws.bytes, stream_of(a), static_cast<unsigned int>(flags));
+  return {status, y, g, u};
+}
+
+std::tuple<int, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> gated_linear_backward(
+    const at::Tensor& grad, const at::Tensor& a, const at::Tensor& b_gate, const at::Tensor& b_up,
+    const at::Tensor& gate, const at::Tensor& up, int activation, bool want_a, bool want_b, bool has_bias,
+    int64_t flags) {
+  check_pair(a, b_gate, b_up, "gated_linear_backward");
+  const c10::cuda::CUDAGuard guard(a.device());
+  const int64_t m = a.size(0), k = a.size(1), n = b_gate.size(1);
+  check_matrix(grad, a, m, n, "grad_output");
+  check_matrix(gate, a, m, n, "gate");
+  check_matrix(up, a, m, n, "up");
+  const at::Tensor dy = by_rows(grad);
+  at::Tensor g = by_rows(gate), u = by_rows(up);
+  if (m > 1 && g.stride(0) != u.stride(0)) {
+    g = g.contiguous();
+    u = u.contiguous();
+  }
+  OptTensor da, dbg, dbu, dbias_g, dbias_u;
+  if (want_a) da = at::empty({m, k}, a.options());
+  if (want_b) {
+    dbg = empty_like_weight(b_gate);
+    dbu = at::empty_strided(dbg->sizes(), dbg->strides(), dbg->options());
+  }
+  if (has_bias) {
+    dbias_g = at::empty({n}, a.options());
+    dbias_u = at::empty({n}, a.options());
+  }
+  const int dtype = dtype_of(a);
+  const Workspace ws(
+      glq_gated_linear_backward_workspace_bytes(dtype, a.data_ptr(), a.stride(0), a.stride(1), b_gate.data_ptr(),
+                                                b_gate.stride(0), b_gate.stride(1), b_up.data_ptr(), b_up.stride(0),
+                                                b_up.stride(1), has_bias ? 1 : 0, m, n, k),
+      a);
+  const int status = glq_gated_linear_backward(
+      dtype, dy.data_ptr(), dy.stride(0), g.data_ptr(), u.data_ptr(), g.stride(0), a.data_ptr(), a.stride(0),
+      a.stride(1), b_gate.data_ptr(), b_gate.stride(0), b_gate.stride(1), b_up.data_ptr(), b_up.stride(0),
+      b_up.stride(1), activation, ptr(da), da.has_value() ? da->stride(0) : 0,
+      ptr(dbg), ptr(dbu), dbg.has_value() ? dbg->stride(0) : 0,
+      dbg.has_value() ? dbg->stride(1) : 0, ptr(dbias_g), ptr(dbias_u), m, n, k,
+      ws.data(), ws.bytes, stream_of(a), static_cast<unsigned int>(flags));
+  return {status, da, dbg, dbu, dbias_g, dbias_u};
+}
+
+void check_norm(const at::Tensor& x, const std::string& op) {
+  if (x.dim() != 2) throw py::value_error(op + " expects a rank-2 tensor");
+  if (!x.is_cuda()) throw py::value_error(op + " requires CUDA tensors");
+  if (x.scalar_type() != at::kHalf && x.scalar_type() != at::kBFloat16) {
+    throw py::value_error("inputs must share dtype float16 or bfloat16");
+  }
+}
+
+std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm(const at::Tensor& x, const OptTensor& weight,
+                                                             const OptTensor& bias, double eps,
+                                                             const OptTensor& output, bool return_stats,
+                                                             int64_t flags) {
+  check_norm(x, "layer_norm");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t m = x.size(0), n = x.size(1);
+  check_vector(weight, x, n, "weight");
+  check_vector(bias, x, n, "bias");
+  const at::Tensor rows = by_rows(x);
+  at::Tensor y = output.has_value() ? *output : at::empty({m, n}, x.options());
+  if (output.has_value()) check_output(y, x, m, n);
+  OptTensor mean, rstd;
+  if (return_stats) {
+    mean = at::empty({m}, x.options().dtype(at::kFloat));
+    rstd = at::empty({m}, x.options().dtype(at::kFloat));
+  }
+  const int status = glq_layer_norm(dtype_of(x), rows.data_ptr(), rows.stride(0), ptr(weight), ptr(bias), eps,
+                                    y.data_ptr(), y.stride(0), return_stats ? mean->data_ptr<float>() : nullptr,
+                                    return_stats ? rstd->data_ptr<float>() : nullptr, m, n, stream_of(x),
+                                    static_cast<unsigned int>(flags));
+  return {status, y, mean, rstd};
+}
+
+std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm_backward(const at::Tensor& grad, const at::Tensor& x,
+                                                                      const at::Tensor& mean, const at::Tensor& rstd,
+                                                                      const OptTensor& weight, bool has_bias,
+                                                                      int64_t flags) {
+  check_norm(x, "layer_norm_backward");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t m = x.size(0), n = x.size(1);
+  check_matrix(grad, x, m, n, "grad_output");
+  check_vector(weight, x, n, "weight");
+  for (const at::Tensor* t : {&mean, &rstd}) {
+    if (t->dim() != 1 || t->size(0) != m || t->device() != x.device() || t->scalar_type() != at::kFloat ||
+        !t->is_contiguous()) {
+      throw py::value_error("mean and rstd are contiguous float32 vectors of one value per row");
+    }
+  }
+  const at::Tensor dy = by_rows(grad), rows = by_rows(x);
+  at::Tensor dx = at::empty({m, n}, x.options());
+  OptTensor dweight, dbias;
+  if (weight.has_value()) dweight = at::empty({n}, x.options());
+  if (has_bias) dbias = at::empty({n}, x.options());
+  const Workspace ws(weight.has_value() || has_bias ? glq_layer_norm_backward_workspace_bytes(m, n) : 0, x);
+  const int status = glq_layer_norm_backward(
+      dtype_of(x), dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), ptr(weight), mean.data_ptr<float>(),
+      rstd.data_ptr<float>(), dx.data_ptr(), dx.stride(0), ptr(dweight),
+      ptr(dbias), m, n, ws.data(), ws.bytes, stream_of(x), static_cast<unsigned int>(flags));
+  return {status, dx, dweight, dbias};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_glq_torch, mod) {
@@ -138,4 +403,10 @@ PYBIND11_MODULE(_glq_torch, mod) {
   mod.def("linear_gather", &linear_gather, py::arg("a"), py::arg("b"), py::arg("bias"), py::arg("epilogue"),
           py::arg("y_ptrs"), py::arg("y_row_stride"), py::arg("y_col_offset"), py::arg("rank"),
           py::arg("signal_ptrs"), py::arg("counter"), py::arg("epoch"), py::arg("split_k"), py::arg("flags"));
+  mod.def("fused_linear", &fused_linear);
+  mod.def("fused_linear_backward", &fused_linear_backward);
+  mod.def("gated_linear", &gated_linear);
+  mod.def("gated_linear_backward", &gated_linear_backward);
+  mod.def("layer_norm", &layer_norm);
+  mod.def("layer_norm_backward", &layer_norm_backward);
 }

@@ -333,6 +333,144 @@ int glq_linear_gather_static(int dtype,
                              uint64_t* const* signal_ranks, int counter_slot, uint64_t epoch,
                              void* stream, unsigned int flags, int* path_out, int* split_out);
 
+/* Activations of the feed-forward operators below. */
+enum glq_activation {
+  GLQ_ACT_NONE = 0,
+  GLQ_ACT_SILU = 1,      /* v * sigmoid(v) */
+  GLQ_ACT_GELU = 2,      /* v * Phi(v), Phi the standard normal distribution */
+  GLQ_ACT_GELU_TANH = 3, /* v / 2 * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) */
+  GLQ_ACT_RELU = 4,
+  GLQ_ACT_COUNT = 5
+};
+
+/*
+ * The feed-forward operators.  No counterpart in the reference, whose only
+ * fused epilogue is bias + SiLU (kernels.py:191-249).  Common rules:
+ *
+ *   - A, B, bias and Y as in glq_linear: A[m, k] and B[k, n] with any
+ *     strides, every other matrix with unit column stride and the given row
+ *     stride (>= its columns; ignored for one row), vectors contiguous.  All
+ *     of one 16-bit type, 2-byte aligned; FP32 sums, one rounding per stored
+ *     value.
+ *   - B with unit k stride (a weight W[N, K] as W^T) and with unit n stride
+ *     are read as they lie, at 16-byte aligned bases and row pitches.  Other
+ *     operands are first copied into the workspace.
+ *   - workspace: device memory of at least the matching *_workspace_bytes()
+ *     bytes, 256-byte aligned (GLQ_ERR_WORKSPACE otherwise; NULL when that is
+ *     0).  It holds nothing between calls: calls that may overlap need
+ *     workspaces of their own.
+ *   - Optional pointers may be NULL; an output that is NULL is not computed.
+ *   - Outputs must not overlap inputs or each other.  flags: enum glq_flags.
+ */
+
+/*
+ * glq_fused_linear -- Z = A B + bias, Y = act(Z) + residual.
+ * bias, residual [M, N] and Z [M, N] (the pre-activations, which the backward
+ * pass reads) are optional.
+ */
+int glq_fused_linear(int dtype, const void* A, int64_t a_row_stride, int64_t a_col_stride,
+                     const void* B, int64_t b_k_stride, int64_t b_n_stride,
+                     const void* bias, int activation,
+                     const void* residual, int64_t residual_row_stride,
+                     void* Z, int64_t z_row_stride, void* Y, int64_t y_row_stride,
+                     int64_t M, int64_t N, int64_t K,
+                     void* workspace, size_t workspace_bytes, void* stream, unsigned int flags);
+
+size_t glq_fused_linear_workspace_bytes(int dtype, const void* A, int64_t a_row_stride, int64_t a_col_stride,
+                                        const void* B, int64_t b_k_stride, int64_t b_n_stride,
+                                        int64_t M, int64_t N, int64_t K);
+
+/*
+ * glq_fused_linear_backward -- gradients of glq_fused_linear from dY [M, N]:
+ *   dZ = dY * act'(Z) (rounded to the 16-bit type: the products' operand),
+ *   dA = dZ B^T, dB = A^T dZ, dbias[n] = sum_m dZ[m, n];
+ * the residual's gradient is dY itself.  Z is required unless activation is
+ * GLQ_ACT_NONE.  dA [M, K] has unit column stride.  dB is [K, N] with
+ * db_k_stride == 1 (the layout of a weight's W^T, row stride db_n_stride) or
+ * db_n_stride == 1.  dA, dB, dbias are each optional.
+ */
+int glq_fused_linear_backward(int dtype, const void* dY, int64_t dy_row_stride,
+                              const void* Z, int64_t z_row_stride,
+                              const void* A, int64_t a_row_stride, int64_t a_col_stride,
+                              const void* B, int64_t b_k_stride, int64_t b_n_stride, int activation,
+                              void* dA, int64_t da_row_stride,
+                              void* dB, int64_t db_k_stride, int64_t db_n_stride, void* dbias,
+                              int64_t M, int64_t N, int64_t K,
+                              void* workspace, size_t workspace_bytes, void* stream, unsigned int flags);
+
+size_t glq_fused_linear_backward_workspace_bytes(int dtype, const void* dY, int64_t dy_row_stride,
+                                                 const void* A, int64_t a_row_stride, int64_t a_col_stride,
+                                                 const void* B, int64_t b_k_stride, int64_t b_n_stride,
+                                                 int activation, int has_bias,
+                                                 int64_t M, int64_t N, int64_t K);
+
+/*
+ * glq_gated_linear -- the gated pair of a feed-forward block in one pass over
+ * A:  G = A Bg + bias_g,  U = A Bu + bias_u,  Y = act(G) * U.
+ * The biases and G, U [M, N] (both or neither, one row stride; what the
+ * backward pass reads) are optional.
+ */
+int glq_gated_linear(int dtype, const void* A, int64_t a_row_stride, int64_t a_col_stride,
+                     const void* Bg, int64_t bg_k_stride, int64_t bg_n_stride,
+                     const void* Bu, int64_t bu_k_stride, int64_t bu_n_stride,
+                     const void* bias_g, const void* bias_u, int activation,
+                     void* G, void* U, int64_t gu_row_stride, void* Y, int64_t y_row_stride,
+                     int64_t M, int64_t N, int64_t K,
+                     void* workspace, size_t workspace_bytes, void* stream, unsigned int flags);
+
+size_t glq_gated_linear_workspace_bytes(int dtype, const void* A, int64_t a_row_stride, int64_t a_col_stride,
+                                        const void* Bg, int64_t bg_k_stride, int64_t bg_n_stride,
+                                        const void* Bu, int64_t bu_k_stride, int64_t bu_n_stride,
+                                        int64_t M, int64_t N, int64_t K);
+
+/*
+ * glq_gated_linear_backward -- gradients of glq_gated_linear from dY [M, N]:
+ *   dG = dY * U * act'(G), dU = dY * act(G) (each rounded to the 16-bit type),
+ *   dA = dG Bg^T + dU Bu^T (summed in FP32, one product),
+ *   dBg = A^T dG, dBu = A^T dU, dbias_g, dbias_u = column sums.
+ * G and U (one row stride) are required.  dBg and dBu are given together,
+ * with one pair of strides as dB above, or not at all; the same holds for
+ * dbias_g and dbias_u.
+ */
+int glq_gated_linear_backward(int dtype, const void* dY, int64_t dy_row_stride,
+                              const void* G, const void* U, int64_t gu_row_stride,
+                              const void* A, int64_t a_row_stride, int64_t a_col_stride,
+                              const void* Bg, int64_t bg_k_stride, int64_t bg_n_stride,
+                              const void* Bu, int64_t bu_k_stride, int64_t bu_n_stride, int activation,
+                              void* dA, int64_t da_row_stride,
+                              void* dBg, void* dBu, int64_t db_k_stride, int64_t db_n_stride,
+                              void* dbias_g, void* dbias_u,
+                              int64_t M, int64_t N, int64_t K,
+                              void* workspace, size_t workspace_bytes, void* stream, unsigned int flags);
+
+size_t glq_gated_linear_backward_workspace_bytes(int dtype, const void* A, int64_t a_row_stride,
+                                                 int64_t a_col_stride,
+                                                 const void* Bg, int64_t bg_k_stride, int64_t bg_n_stride,
+                                                 const void* Bu, int64_t bu_k_stride, int64_t bu_n_stride,
+                                                 int has_bias, int64_t M, int64_t N, int64_t K);
+
+/*
+ * glq_layer_norm -- Y[m, :] = (X[m, :] - mean_m) * rstd_m * weight + bias with
+ * mean_m the row's mean and rstd_m = 1 / sqrt(mean((X[m, :] - mean_m)^2) + eps).
+ * weight and bias [N] are optional; mean and rstd (FP32 [M], both or neither)
+ * are what the backward pass reads.
+ */
+int glq_layer_norm(int dtype, const void* X, int64_t x_row_stride, const void* weight, const void* bias, double eps,
+                   void* Y, int64_t y_row_stride, float* mean, float* rstd, int64_t M, int64_t N,
+                   void* stream, unsigned int flags);
+
+/*
+ * glq_layer_norm_backward -- with xhat = (X - mean) * rstd and g = dY * weight:
+ *   dX = rstd * (g - mean(g) - xhat * mean(g * xhat)) per row,
+ *   dweight = sum_m dY * xhat, dbias = sum_m dY (each optional; fixed order).
+ */
+int glq_layer_norm_backward(int dtype, const void* dY, int64_t dy_row_stride, const void* X, int64_t x_row_stride,
+                            const void* weight, const float* mean, const float* rstd,
+                            void* dX, int64_t dx_row_stride, void* dweight, void* dbias, int64_t M, int64_t N,
+                            void* workspace, size_t workspace_bytes, void* stream, unsigned int flags);
+
+size_t glq_layer_norm_backward_workspace_bytes(int64_t M, int64_t N);
+
 /* Names of paths and statuses (static strings, never NULL). */
 const char* glq_path_name(int path);
 const char* glq_status_string(int status);
