@@ -13,6 +13,7 @@
 
 #include "glq_ffn.h"
 #include "glq_internal.h"
+#include "glq_rows.h"
 
 namespace glq {
 namespace {
@@ -57,7 +58,8 @@ int device_state(DeviceState** out) {
     void* word = nullptr;
     if (cudaGetSymbolAddress(&word, g_device_error_word) != cudaSuccess ||
         tc_prepare_device() != cudaSuccess || gemv_prepare_device() != cudaSuccess ||
-        pair_prepare_device() != cudaSuccess || skinny_prepare_device() != cudaSuccess) {
+        pair_prepare_device() != cudaSuccess || skinny_prepare_device() != cudaSuccess ||
+        rows_prepare_device() != cudaSuccess) {
       cudaGetLastError();
       st.status = GLQ_ERR_CUDA;
       return;

@@ -586,6 +586,7 @@ int glq_layer_norm(int dtype, const void* X, int64_t x_row_stride, const void* w
   a.rows = M;
   a.cols = static_cast<int>(N);
   a.eps = static_cast<float>(eps);
+  a.err = err;
   return glq::status_of(glq::launch_norm(dtype, a, sm_count, flags, static_cast<cudaStream_t>(stream)));
 }
 
@@ -637,6 +638,7 @@ int glq_layer_norm_backward(int dtype, const void* dY, int64_t dy_row_stride, co
   a.ld_dx = dx_row_stride;
   a.rows = M;
   a.cols = static_cast<int>(N);
+  a.err = err;
   return glq::status_of(glq::launch_norm_backward(dtype, a, dweight, dbias, sm_count, flags, s));
 }
 

@@ -11,145 +11,324 @@
 #include <algorithm>
 
 #include "glq_act.cuh"
+#include "glq_internal.h"
 #include "glq_ptx.cuh"
 #include "glq_rows.h"
 
 namespace glq {
 namespace {
 
-// Eight consecutive elements of a row as floats; vec: 16-byte aligned and
-// all inside, else `valid` of them element by element (the rest 0).
+// Eight consecutive 16-bit elements of a row.  align: bytes that every row's
+// start is a multiple of (16, 8, 4 or 2); fewer than 8 valid elements are read
+// and written one by one (the rest 0).
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int valid, float (&v)[8]) {
-  if (vec) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+__device__ __forceinline__ uint4 load8_raw(const T* p, int align, int valid) {
+  if (valid >= 8 && align == 16) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4];
+  if (valid >= 8 && align == 8) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p), y = *reinterpret_cast<const uint2*>(p + 4);
+    w[0] = x.x, w[1] = x.y, w[2] = y.x, w[3] = y.y;
+  } else if (valid >= 8 && align == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint32_t*>(p + 2 * i);
+  } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = Elem16<T>::to_f2(w[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+      const uint32_t lo = 2 * i < valid ? q[2 * i] : 0u, hi = 2 * i + 1 < valid ? q[2 * i + 1] : 0u;
+      w[i] = lo | (hi << 16);
     }
-  } else {
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store8_raw(T* p, int align, int valid, const uint4& x) {
+  if (valid >= 8 && align == 16) {
+    *reinterpret_cast<uint4*>(p) = x;
+    return;
+  }
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  if (valid >= 8 && align == 8) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(p + 4) = make_uint2(w[2], w[3]);
+  } else if (valid >= 8 && align == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < valid ? Elem16<T>::to_f(p[i]) : 0.0f;
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(p + 2 * i) = w[i];
+  } else {
+    uint16_t* q = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < valid) q[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// The same as floats.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int align, int valid, float (&v)[8]) {
+  const uint4 x = load8_raw(p, align, valid);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Elem16<T>::to_f2(w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, bool vec, int valid, const float (&v)[8]) {
-  if (vec) {
-    uint4 x;
-    x.x = Elem16<T>::from_f2(v[0], v[1]);
-    x.y = Elem16<T>::from_f2(v[2], v[3]);
-    x.z = Elem16<T>::from_f2(v[4], v[5]);
-    x.w = Elem16<T>::from_f2(v[6], v[7]);
-    *reinterpret_cast<uint4*>(p) = x;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i < valid) p[i] = Elem16<T>::from_f(v[i]);
-    }
-  }
+__device__ __forceinline__ void store8(T* p, int align, int valid, const float (&v)[8]) {
+  store8_raw(p, align, valid,
+             make_uint4(Elem16<T>::from_f2(v[0], v[1]), Elem16<T>::from_f2(v[2], v[3]), Elem16<T>::from_f2(v[4], v[5]),
+                        Elem16<T>::from_f2(v[6], v[7])));
 }
 
-// Sum of N values over the G threads of a row (all threads of the block call
-// it; blocks of more than a warp per row use shared memory, red[2][32 N]).
+// Sum of N values over the G threads of a row.  Groups of more than a warp
+// join through red[2][G / 32][N], their own, behind the group's named barrier;
+// every thread adds the warps' sums in the same order.
 template <int G, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float* red, int& phase) {
+__device__ __forceinline__ void row_sum(float (&v)[N], float* red, int& phase, int group) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   }
   if constexpr (G > 32) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float* buf = red + phase * 32 * N;  // two buffers: one barrier per sum
+    constexpr int kWarps = G / 32;
+    const int warp = (threadIdx.x % G) >> 5, lane = threadIdx.x & 31;
+    float* buf = red + phase * kWarps * N;  // two buffers: one barrier per sum
     phase ^= 1;
     if (lane == 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) buf[warp * N + i] = v[i];
     }
-    __syncthreads();
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(G) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < G / 32; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] += buf[w * N + i];
     }
   }
 }
 
+// Two floats in one 64-bit register pair: one instruction adds or multiplies
+// both, which the row kernels need to stay bound by memory.
+using Two = unsigned long long;
+
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves(Two a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& x, Two (&v)[4]) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Elem16<T>::to_f2(w[i]);
+    v[i] = two(f.x, f.y);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack(const Two (&v)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = halves(v[i]);
+    w[i] = Elem16<T>::from_f2(f.x, f.y);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Rows on their way to a group of threads: STAGES slots of ROWS tensors' rows
+// in shared memory, filled by bulk copies that the group's first thread
+// starts, so the bytes in flight do not depend on registers or on how long a
+// row's joins take.  An expired wait raises the error word and lets the group
+// go on (with what the slot holds), so no barrier is missed.
+template <int ROWS, int STAGES>
+struct RowRing {
+  uint32_t slots, bars;  // shared-memory addresses
+  uint32_t row_bytes;
+  unsigned int* err;
+  uint64_t policy;
+  int fill = 0, use = 0;
+
+  __device__ __forceinline__ void start(const void* const (&rows)[ROWS]) {
+    const int s = fill % STAGES;
+    ptx::mbar_arrive_expect_tx(bars + 8 * s, ROWS * row_bytes);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      ptx::bulk_load_1d(slots + (s * ROWS + i) * row_bytes, rows[i], row_bytes, bars + 8 * s, policy);
+    }
+    ++fill;
+  }
+  // Waits for the next slot and returns its address.
+  __device__ uint32_t wait() {
+    const int s = use % STAGES;
+    if (!ptx::mbar_wait_bounded(bars + 8 * s, (use / STAGES) & 1, nullptr, kWaitBudgetNs)) {
+      atomicOr(err, kErrTimeoutProducer);
+    }
+    ++use;
+    return slots + s * ROWS * row_bytes;
+  }
+};
+
+__device__ __forceinline__ uint4 ld_smem_v4(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+
 // ---------------------------------------------------------------- layer norm
 //
 // A row is held in registers by G threads (V vectors of 8 each), so x is read
 // once and the variance is the mean of the squared deviations from the mean
-// (no cancellation of large squares).  Rows of up to 512 columns take one
-// warp each, four rows per block.
+// (no cancellation of large squares).  What bounds it is HBM, as long as loads
+// are in flight while a row's two joins wait and the instructions per element
+// stay below about a dozen: persistent groups of threads walk rows group,
+// + groups, ..., each requesting its next row before it reduces the present
+// one (one row per block instead: 159 us at 16384 x 8192; rows by bulk copies
+// through shared memory: 123 us, the joins' latency then has too few groups
+// per SM to hide behind), and arithmetic is paired.  VEC: rows of whole
+// 16-byte vectors; other rows are read where they are used.
 
-template <int G>
-constexpr int kRowsPerBlock = G == 32 ? 4 : 1;
+constexpr int kNormThreads = 256;
 
-template <typename T, int G, int V>
-__global__ void __launch_bounds__(G * kRowsPerBlock<G>)
-    norm_kernel(const NormArgs a) {
-  __shared__ float red[2 * 32];
+template <typename T, int G, int V, bool VEC>
+__global__ void __launch_bounds__(G < kNormThreads ? kNormThreads : G, G < 512 ? 3 : 1) norm_kernel(const NormArgs a) {
+  constexpr int kGroups = G < kNormThreads ? kNormThreads / G : 1;  // rows per block at a time
+  __shared__ float red[kGroups * 2 * (G / 32)];
   int phase = 0;
-  const int in_row = threadIdx.x % G;
-  const int first = blockIdx.x * kRowsPerBlock<G> + threadIdx.x / G;
+  const int group = threadIdx.x / G;
+  const int c0 = (threadIdx.x % G) * 8;
   const int cols = a.cols;
   const float inv = 1.0f / static_cast<float>(cols);
+  float* my_red = red + group * 2 * (G / 32);
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const T* weight = static_cast<const T*>(a.weight);
   const T* bias = static_cast<const T*>(a.bias);
-  for (long long r0 = first; r0 - threadIdx.x / G < a.rows; r0 += static_cast<long long>(gridDim.x) * kRowsPerBlock<G>) {
-    const bool live = r0 < a.rows;  // whole warps: G >= 32
-    const T* x = static_cast<const T*>(a.x) + r0 * a.ld_x;
-    float v[V][8];
-    float sum[1] = {0.0f};
+  const T* x = static_cast<const T*>(a.x);
+  const long long step = static_cast<long long>(gridDim.x) * kGroups;
+  long long r = static_cast<long long>(blockIdx.x) * kGroups + group;
+  uint4 next[VEC ? V : 1];
+  auto request = [&](long long row) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = c0 + j * G * 8;
+        next[j] = c < cols ? ptx::ldg_stream_v4(x + row * a.ld_x + c) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  if (r < a.rows) request(r);
+  for (; r < a.rows; r += step) {
+    Two v[V][4];
+    Two acc = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (j * G + in_row) * 8;
-      load8(x + c, live && a.vec && c < cols, live ? cols - c : 0, v[j]);
+      if constexpr (VEC) {
+        unpack<T>(next[j], v[j]);
+      } else {
+        const int c = c0 + j * G * 8;
+        float f[8];
+        load8(x + r * a.ld_x + c, a.align, cols - c, f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[0] += v[j][i];
+        for (int i = 0; i < 4; ++i) v[j][i] = two(f[2 * i], f[2 * i + 1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc = add2(acc, v[j][i]);
     }
-    row_sum<G>(sum, red, phase);
+    if (r + step < a.rows) request(r + step);
+    float sum[1] = {halves(acc).x + halves(acc).y};
+    row_sum<G>(sum, my_red, phase, group);
     const float mean = sum[0] * inv;
-    float sq[1] = {0.0f};
+    const Two minus_mean = two(-mean, -mean);
+    acc = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (j * G + in_row) * 8;
+      const int c = c0 + j * G * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[j][i] -= mean;
-        if (c + i < cols) sq[0] += v[j][i] * v[j][i];
+      for (int i = 0; i < 4; ++i) {
+        v[j][i] = add2(v[j][i], minus_mean);
+        if (!VEC && c + 2 * i + 1 >= cols) {  // past the end, or the last of an odd number
+          v[j][i] = two(c + 2 * i < cols ? halves(v[j][i]).x : 0.0f, 0.0f);
+        }
+        if (!VEC || c < cols) acc = fma2(v[j][i], v[j][i], acc);
       }
     }
-    row_sum<G>(sq, red, phase);
-    const float rstd = rsqrtf(sq[0] * inv + a.eps);
-    if (!live) continue;
-    T* y = static_cast<T*>(a.y) + r0 * a.ld_y;
+    sum[0] = halves(acc).x + halves(acc).y;
+    row_sum<G>(sum, my_red, phase, group);
+    const float rstd = rsqrtf(sum[0] * inv + a.eps);
+    const Two scale = two(rstd, rstd);
+    T* y = static_cast<T*>(a.y) + r * a.ld_y;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (j * G + in_row) * 8;
+      const int c = c0 + j * G * 8;
       if (c >= cols) continue;
-      float w[8], b[8];
-      if (weight != nullptr) load8(weight + c, a.vec_w, cols - c, w);
-      if (bias != nullptr) load8(bias + c, a.vec_w, cols - c, b);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[j][i] *= rstd;
-        if (weight != nullptr) v[j][i] *= w[i];
-        if (bias != nullptr) v[j][i] += b[i];
+      for (int i = 0; i < 4; ++i) v[j][i] = mul2(v[j][i], scale);
+      if constexpr (VEC) {  // (align_w is 16)
+        Two w[4];
+        if (weight != nullptr) {
+          unpack<T>(*reinterpret_cast<const uint4*>(weight + c), w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[j][i] = mul2(v[j][i], w[i]);
+        }
+        if (bias != nullptr) {
+          unpack<T>(*reinterpret_cast<const uint4*>(bias + c), w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[j][i] = add2(v[j][i], w[i]);
+        }
+        *reinterpret_cast<uint4*>(y + c) = pack<T>(v[j]);
+      } else {
+        float f[8], w[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[2 * i] = halves(v[j][i]).x;
+          f[2 * i + 1] = halves(v[j][i]).y;
+        }
+        if (weight != nullptr) {
+          load8(weight + c, a.align_w, cols - c, w);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] *= w[i];
+        }
+        if (bias != nullptr) {
+          load8(bias + c, a.align_w, cols - c, w);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] += w[i];
+        }
+        store8(y + c, a.align, cols - c, f);
       }
-      store8(y + c, a.vec, cols - c, v[j]);
     }
-    if (in_row == 0 && a.mean != nullptr) {
-      a.mean[r0] = mean;
-      a.rstd[r0] = rstd;
+    if (c0 == 0 && a.mean != nullptr) {
+      a.mean[r] = mean;
+      a.rstd[r] = rstd;
     }
   }
 }
@@ -170,30 +349,30 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a) {
     T* y = static_cast<T*>(a.y) + r * a.ld_y;
     float sum[1] = {0.0f}, sq[1] = {0.0f}, v[8];
     for (int c = threadIdx.x * 8; c < a.cols; c += 1024 * 8) {
-      load8(x + c, a.vec, a.cols - c, v);
+      load8(x + c, a.align, a.cols - c, v);
       for (int i = 0; i < 8; ++i) sum[0] += v[i];
     }
-    row_sum<1024>(sum, red, phase);
+    row_sum<1024>(sum, red, phase, 0);
     const float mean = sum[0] * inv;
     for (int c = threadIdx.x * 8; c < a.cols; c += 1024 * 8) {
-      load8(x + c, a.vec, a.cols - c, v);
+      load8(x + c, a.align, a.cols - c, v);
       for (int i = 0; i < 8; ++i) {
         if (c + i < a.cols) sq[0] += (v[i] - mean) * (v[i] - mean);
       }
     }
-    row_sum<1024>(sq, red, phase);
+    row_sum<1024>(sq, red, phase, 0);
     const float rstd = rsqrtf(sq[0] * inv + a.eps);
     for (int c = threadIdx.x * 8; c < a.cols; c += 1024 * 8) {
       float w[8], b[8];
-      load8(x + c, a.vec, a.cols - c, v);
-      if (weight != nullptr) load8(weight + c, a.vec_w, a.cols - c, w);
-      if (bias != nullptr) load8(bias + c, a.vec_w, a.cols - c, b);
+      load8(x + c, a.align, a.cols - c, v);
+      if (weight != nullptr) load8(weight + c, a.align_w, a.cols - c, w);
+      if (bias != nullptr) load8(bias + c, a.align_w, a.cols - c, b);
       for (int i = 0; i < 8; ++i) {
         v[i] = (v[i] - mean) * rstd;
         if (weight != nullptr) v[i] *= w[i];
         if (bias != nullptr) v[i] += b[i];
       }
-      store8(y + c, a.vec, a.cols - c, v);
+      store8(y + c, a.align, a.cols - c, v);
     }
     if (threadIdx.x == 0 && a.mean != nullptr) {
       a.mean[r] = mean;
@@ -205,83 +384,158 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a) {
 // Backward.  With xhat = (x - mean) rstd and g = dy w:
 //   dx = rstd (g - mean(g) - xhat mean(g xhat)),  dw = sum_r dy xhat,
 //   db = sum_r dy.
-// A block walks rows blockIdx.x, + gridDim.x, ... and keeps its columns' dw
-// and db sums in registers; partial rows go to part[block row][2][cols].
-template <typename T, int G, int V>
-__global__ void __launch_bounds__(G * kRowsPerBlock<G>)
-    norm_backward_kernel(const NormBackwardArgs a) {
-  __shared__ float red[2 * 32 * 2];
+// One block per SM.  Its groups of G threads walk the rows, the next ones on
+// their way to shared memory (RowRing) and their statistics to registers, and
+// keep their columns' dw and db sums in registers; a row is read twice from
+// its slot (sums, then dx).  The weight waits as floats in shared memory.  At
+// the end the groups' sums are added in order in shared memory, so a block
+// leaves one partial row: part[block][2][part_cols].  (16384 x 8192: 243 us
+// with rows requested into registers and unpaired arithmetic; two rows per
+// join with half the columns per thread spills and is slower on most widths.)
+constexpr int kRowThreads = 512;
+template <int G>
+constexpr int kBackwardStages = G < 512 ? 3 : 2;
+
+template <typename T, int G, int V, bool VEC>
+__global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const NormBackwardArgs a) {
+  constexpr int kGroups = kRowThreads / G;
+  constexpr int kStages = kBackwardStages<G>;
+  __shared__ float red[kGroups * 2 * (G / 32) * 2];
+  __shared__ alignas(8) uint64_t bars[kGroups * kStages];
+  extern __shared__ __align__(128) uint8_t dyn_smem[];  // weight, rings; at the end: float [groups][2][part_cols]
   int phase = 0;
-  const int in_row = threadIdx.x % G;
-  const int sub = threadIdx.x / G;
+  const int group = threadIdx.x / G;
+  const int c0 = (threadIdx.x % G) * 8;
   const int cols = a.cols;
+  float* weight = reinterpret_cast<float*>(dyn_smem);
   const float inv = 1.0f / static_cast<float>(cols);
+  float* my_red = red + group * 2 * (G / 32) * 2;
+  if (VEC && threadIdx.x < kGroups * kStages) ptx::mbar_init(ptx::smem_addr(&bars[threadIdx.x]), 1);
+  ptx::fence_mbar_init();
+  __syncthreads();
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const T* weight = static_cast<const T*>(a.weight);
-  float w[V][8], dw[V][8], db[V][8];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int c = (j * G + in_row) * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      w[j][i] = 1.0f;
-      dw[j][i] = 0.0f;
-      db[j][i] = 0.0f;
-    }
-    if (weight != nullptr && c < cols) load8(weight + c, a.vec_w, cols - c, w[j]);
+  const T* x = static_cast<const T*>(a.x);
+  const T* dy = static_cast<const T*>(a.dy);
+  Two dw[V][4] = {}, db[V][4] = {};
+  const long long step = static_cast<long long>(gridDim.x) * kGroups;
+  long long r = static_cast<long long>(blockIdx.x) * kGroups + group;
+  RowRing<2, kStages> ring;
+  ring.row_bytes = static_cast<uint32_t>(cols) * 2u;
+  ring.slots = ptx::smem_addr(weight + a.part_cols) + group * kStages * 2 * ring.row_bytes;
+  ring.bars = ptx::smem_addr(&bars[group * kStages]);
+  ring.err = a.err;
+  ring.policy = ptx::policy_evict_first();
+  auto start = [&](long long row) { ring.start({x + row * a.ld_x, dy + row * a.ld_dy}); };
+  if (VEC && c0 == 0) {
+    for (int i = 0; i < kStages && r + i * step < a.rows; ++i) start(r + i * step);
   }
-  for (long long r0 = static_cast<long long>(blockIdx.x) * kRowsPerBlock<G> + sub; r0 - sub < a.rows;
-       r0 += static_cast<long long>(gridDim.x) * kRowsPerBlock<G>) {
-    const bool live = r0 < a.rows;
-    const T* x = static_cast<const T*>(a.x) + r0 * a.ld_x;
-    const T* dy = static_cast<const T*>(a.dy) + r0 * a.ld_dy;
-    const float mean = live ? a.mean[r0] : 0.0f;
-    const float rstd = live ? a.rstd[r0] : 0.0f;
-    float xh[V][8], g[V][8];
-    float sum[2] = {0.0f, 0.0f};  // of g xhat and of g
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  if (r < a.rows) {
+    next_mean = a.mean[r];
+    next_rstd = a.rstd[r];
+  }
+  {
+    const T* from = static_cast<const T*>(a.weight);
+    for (int c = threadIdx.x * 8; c < cols; c += kRowThreads * 8) {
+      float f[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+      if (from != nullptr) load8(from + c, a.align_w, cols - c, f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (j * G + in_row) * 8;
-      load8(x + c, live && a.vec && c < cols, live ? cols - c : 0, xh[j]);
-      load8(dy + c, live && a.vec && c < cols, live ? cols - c : 0, g[j]);
+      for (int i = 0; i < 8; ++i) weight[c + i] = f[i];  // part_cols is a multiple of 8
     }
+  }
+  __syncthreads();
+  for (; r < a.rows; r += step) {
+    const float rstd = next_rstd;
+    const float shift = -next_mean * rstd;  // xhat = x rstd + shift
+    if (r + step < a.rows) {
+      next_mean = a.mean[r + step];
+      next_rstd = a.rstd[r + step];
+    }
+    [[maybe_unused]] const uint32_t slot = VEC ? ring.wait() : 0u;
+    // x and dy of vector j (0 past the row's end).
+    auto at = [&](int j, Two(&xv)[4], Two(&gv)[4]) {
+      const int c = c0 + j * G * 8;
+      if constexpr (VEC) {
+        unpack<T>(ld_smem_v4(slot + 2 * c), xv);
+        unpack<T>(ld_smem_v4(slot + ring.row_bytes + 2 * c), gv);
+      } else {
+        unpack<T>(load8_raw(x + r * a.ld_x + c, a.align, cols - c), xv);
+        unpack<T>(load8_raw(dy + r * a.ld_dy + c, a.align, cols - c), gv);
+      }
+    };
+    auto weights = [&](int j, Two(&w)[4]) {
+      const ulonglong2* p = reinterpret_cast<const ulonglong2*>(weight + c0 + j * G * 8);
+      const ulonglong2 lo = p[0], hi = p[1];
+      w[0] = lo.x, w[1] = lo.y, w[2] = hi.x, w[3] = hi.y;
+    };
+    const Two rstd2 = two(rstd, rstd), shift2 = two(shift, shift);
+    Two s0 = 0, s1 = 0;  // sums of dy w xhat and of dy w
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+      if (c0 + j * G * 8 >= cols) continue;
+      Two xv[4], g[4], w[4];
+      at(j, xv, g);
+      weights(j, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        xh[j][i] = (xh[j][i] - mean) * rstd;  // columns past the end: g is 0
-        dw[j][i] += g[j][i] * xh[j][i];
-        db[j][i] += g[j][i];
-        g[j][i] *= w[j][i];
-        sum[0] += g[j][i] * xh[j][i];
-        sum[1] += g[j][i];
+      for (int i = 0; i < 4; ++i) {
+        const Two t = mul2(g[i], fma2(xv[i], rstd2, shift2));
+        dw[j][i] = add2(dw[j][i], t);
+        db[j][i] = add2(db[j][i], g[i]);
+        s0 = fma2(t, w[i], s0);
+        s1 = fma2(g[i], w[i], s1);
       }
     }
-    row_sum<G>(sum, red, phase);
-    const float c1 = sum[0] * inv, c2 = sum[1] * inv;
-    if (!live) continue;
-    T* dx = static_cast<T*>(a.dx) + r0 * a.ld_dx;
+    float sum[2] = {halves(s0).x + halves(s0).y, halves(s1).x + halves(s1).y};
+    row_sum<G>(sum, my_red, phase, group);
+    // Past this join the whole group is done with the row before this one:
+    // its slot takes the row kStages - 1 ahead.
+    if (VEC && c0 == 0 && ring.use > 1 && r + (kStages - 1) * step < a.rows) start(r + (kStages - 1) * step);
+    // dx = (rstd w) dy - rstd mean(g xhat) xhat - rstd mean(g)
+    const float k1 = -rstd * (sum[0] * inv), k2 = -rstd * (sum[1] * inv);
+    const float level1 = fmaf(shift, k1, k2);
+    const Two slope = two(k1 * rstd, k1 * rstd), level = two(level1, level1);
+    T* dx = static_cast<T*>(a.dx) + r * a.ld_dx;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (j * G + in_row) * 8;
+      const int c = c0 + j * G * 8;
       if (c >= cols) continue;
+      Two xv[4], g[4], w[4];
+      at(j, xv, g);
+      weights(j, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[j][i] = (g[j][i] - c2 - xh[j][i] * c1) * rstd;
-      store8(dx + c, a.vec, cols - c, g[j]);
+      for (int i = 0; i < 4; ++i) g[i] = fma2(g[i], mul2(w[i], rstd2), fma2(xv[i], slope, level));
+      if constexpr (VEC) {
+        *reinterpret_cast<uint4*>(dx + c) = pack<T>(g);
+      } else {
+        store8_raw(dx + c, a.align, cols - c, pack<T>(g));
+      }
     }
   }
   if (a.part == nullptr) return;
-  float* part = a.part + (static_cast<long long>(blockIdx.x) * kRowsPerBlock<G> + sub) * 2 * a.part_cols;
+  float* part = a.part + static_cast<long long>(blockIdx.x) * 2 * a.part_cols;
+  // One group writes its sums; several leave them side by side in shared
+  // memory (over their drained rings), added per column in group order.
+  float* joined = reinterpret_cast<float*>(dyn_smem);
+  if (kGroups > 1) __syncthreads();
+  float* to = kGroups > 1 ? joined + static_cast<size_t>(group) * 2 * a.part_cols : part;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int c = (j * G + in_row) * 8;
+    const int c = c0 + j * G * 8;
     if (c >= cols) continue;
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {  // part_cols is a multiple of 8
-      *reinterpret_cast<float4*>(part + c + i) = make_float4(dw[j][i], dw[j][i + 1], dw[j][i + 2], dw[j][i + 3]);
-      *reinterpret_cast<float4*>(part + a.part_cols + c + i) =
-          make_float4(db[j][i], db[j][i + 1], db[j][i + 2], db[j][i + 3]);
+    for (int i = 0; i < 4; ++i) {  // part_cols is a multiple of 8
+      *reinterpret_cast<Two*>(to + c + 2 * i) = dw[j][i];
+      *reinterpret_cast<Two*>(to + a.part_cols + c + 2 * i) = db[j][i];
+    }
+  }
+  if (kGroups > 1) {
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * a.part_cols; c += kRowThreads) {
+      float t = joined[c];
+#pragma unroll
+      for (int g = 1; g < kGroups; ++g) t += joined[static_cast<size_t>(g) * 2 * a.part_cols + c];
+      part[c] = t;
     }
   }
 }
@@ -302,26 +556,26 @@ __global__ void __launch_bounds__(1024) norm_backward_long_kernel(const NormBack
     const float mean = a.mean[r], rstd = a.rstd[r];
     float sum[2] = {0.0f, 0.0f}, xv[8], g[8], w[8];
     for (int c = threadIdx.x * 8; c < a.cols; c += 1024 * 8) {
-      load8(x + c, a.vec, a.cols - c, xv);
-      load8(dy + c, a.vec, a.cols - c, g);
-      if (weight != nullptr) load8(weight + c, a.vec_w, a.cols - c, w);
+      load8(x + c, a.align, a.cols - c, xv);
+      load8(dy + c, a.align, a.cols - c, g);
+      if (weight != nullptr) load8(weight + c, a.align_w, a.cols - c, w);
       for (int i = 0; i < 8; ++i) {
         const float gw = weight != nullptr ? g[i] * w[i] : g[i];
         sum[0] += gw * (xv[i] - mean) * rstd;
         sum[1] += gw;
       }
     }
-    row_sum<1024>(sum, red, phase);
+    row_sum<1024>(sum, red, phase, 0);
     const float c1 = sum[0] * inv, c2 = sum[1] * inv;
     for (int c = threadIdx.x * 8; c < a.cols; c += 1024 * 8) {
-      load8(x + c, a.vec, a.cols - c, xv);
-      load8(dy + c, a.vec, a.cols - c, g);
-      if (weight != nullptr) load8(weight + c, a.vec_w, a.cols - c, w);
+      load8(x + c, a.align, a.cols - c, xv);
+      load8(dy + c, a.align, a.cols - c, g);
+      if (weight != nullptr) load8(weight + c, a.align_w, a.cols - c, w);
       for (int i = 0; i < 8; ++i) {
         const float gw = weight != nullptr ? g[i] * w[i] : g[i];
         g[i] = (gw - c2 - (xv[i] - mean) * rstd * c1) * rstd;
       }
-      store8(dx + c, a.vec, a.cols - c, g);
+      store8(dx + c, a.align, a.cols - c, g);
     }
   }
 }
@@ -338,8 +592,8 @@ __global__ void __launch_bounds__(128) norm_columns_kernel(const NormBackwardArg
   float dw[8] = {}, db[8] = {};
   for (long long r = lo; r < hi; ++r) {
     float xv[8], g[8];
-    load8(static_cast<const T*>(a.x) + r * a.ld_x + c, a.vec, a.cols - c, xv);
-    load8(static_cast<const T*>(a.dy) + r * a.ld_dy + c, a.vec, a.cols - c, g);
+    load8(static_cast<const T*>(a.x) + r * a.ld_x + c, a.align, a.cols - c, xv);
+    load8(static_cast<const T*>(a.dy) + r * a.ld_dy + c, a.align, a.cols - c, g);
     const float mean = a.mean[r], rstd = a.rstd[r];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -357,11 +611,14 @@ __global__ void __launch_bounds__(128) norm_columns_kernel(const NormBackwardArg
 
 // ---------------------------------------------------------------- column sums
 //
-// out[c] = sum over p of part[p][c], in order of p inside each of 8 strided
-// ranges, then the 8 in order.  32 columns x 8 ranges per block.
+// out[c] = sum over p of part[p][c], in order of p inside each of 16 strided
+// ranges, then the 16 in order.  32 columns x 16 ranges per block; a range's
+// loads are requested eight at a time (bound by their latency).
+constexpr int kSumRanges = 16;
+
 template <typename T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const ColumnSumArgs a) {
-  __shared__ float sums[8][33];
+__global__ void __launch_bounds__(32 * kSumRanges) column_sum_kernel(const ColumnSumArgs a) {
+  __shared__ float sums[kSumRanges][33];
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
@@ -370,15 +627,18 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const ColumnSumArgs a) 
   float s = 0.0f;
   if (c < a.cols) {
     const float* p = a.part + static_cast<long long>(which) * a.part_cols + c;
-    for (int i = q; i < a.parts; i += 8) s += p[static_cast<long long>(i) * a.sums * a.part_cols];
+    const long long step = static_cast<long long>(a.sums) * a.part_cols;
+#pragma unroll 8
+    for (int i = q; i < a.parts; i += kSumRanges) s += p[i * step];
   }
   sums[q][lane] = s;
   __syncthreads();
-  if (q == 0 && c < a.cols && a.out[which] != nullptr) {
+  T* out = static_cast<T*>(which == 0 ? a.out[0] : a.out[1]);
+  if (q == 0 && c < a.cols && out != nullptr) {
     float t = sums[0][lane];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) t += sums[i][lane];
-    static_cast<T*>(a.out[which])[c] = Elem16<T>::from_f(t);
+    for (int i = 1; i < kSumRanges; ++i) t += sums[i][lane];
+    out[c] = Elem16<T>::from_f(t);
   }
 }
 
@@ -404,9 +664,9 @@ __global__ void __launch_bounds__(128) act_backward_kernel(const ActBackwardArgs
 #pragma unroll 2
     for (long long r = lo; r < hi; ++r) {
       float g[8], z[8], u[8], d0[8], d1[8];
-      load8(static_cast<const T*>(a.dy) + r * a.ld_dy + c, a.vec_dy, valid, g);
-      if (GATED || ACT != GLQ_ACT_NONE) load8(static_cast<const T*>(a.pre[0]) + r * a.ld_pre + c, a.vec_pre, valid, z);
-      if (GATED) load8(static_cast<const T*>(a.pre[1]) + r * a.ld_pre + c, a.vec_pre, valid, u);
+      load8(static_cast<const T*>(a.dy) + r * a.ld_dy + c, a.align_dy, valid, g);
+      if (GATED || ACT != GLQ_ACT_NONE) load8(static_cast<const T*>(a.pre[0]) + r * a.ld_pre + c, a.align_pre, valid, z);
+      if (GATED) load8(static_cast<const T*>(a.pre[1]) + r * a.ld_pre + c, a.align_pre, valid, u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float value = 0.0f, slope = 1.0f;
@@ -421,8 +681,8 @@ __global__ void __launch_bounds__(128) act_backward_kernel(const ActBackwardArgs
         s0[i] += i < valid ? d0[i] : 0.0f;
       }
       if (a.dz[0] != nullptr) {  // null: column sums only
-        store8(static_cast<T*>(a.dz[0]) + r * a.ld_dz + c, a.vec_dz, valid, d0);
-        if (GATED) store8(static_cast<T*>(a.dz[1]) + r * a.ld_dz + c, a.vec_dz, valid, d1);
+        store8(static_cast<T*>(a.dz[0]) + r * a.ld_dz + c, a.align_dz, valid, d0);
+        if (GATED) store8(static_cast<T*>(a.dz[1]) + r * a.ld_dz + c, a.align_dz, valid, d1);
       }
     }
   });
@@ -440,8 +700,10 @@ __global__ void __launch_bounds__(128) act_backward_kernel(const ActBackwardArgs
 // ---------------------------------------------------------------- host
 
 template <typename Kernel, typename Args>
-cudaError_t launch(Kernel kernel, dim3 grid, int threads, const Args& args, unsigned int flags, cudaStream_t s) {
+cudaError_t launch(Kernel kernel, dim3 grid, int threads, size_t smem, const Args& args, unsigned int flags,
+                   cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = smem;
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.stream = s;
@@ -453,66 +715,108 @@ cudaError_t launch(Kernel kernel, dim3 grid, int threads, const Args& args, unsi
   return cudaLaunchKernelEx(&cfg, kernel, args);
 }
 
-bool vec_rows(const void* p, int64_t ld, int64_t cols) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0 && cols % 8 == 0;
-}
-
-// Threads per row and vectors per thread of the register kernels.
-template <typename T, template <typename, int, int> class Launch, typename Args>
-cudaError_t by_columns(const Args& a, int grid, unsigned int flags, cudaStream_t s) {
-  if (a.cols <= 256) return Launch<T, 32, 1>::run(a, grid, flags, s);
-  if (a.cols <= 512) return Launch<T, 32, 2>::run(a, grid, flags, s);
-  if (a.cols <= 1024) return Launch<T, 128, 1>::run(a, grid, flags, s);
-  if (a.cols <= 2048) return Launch<T, 128, 2>::run(a, grid, flags, s);
-  if (a.cols <= 4096) return Launch<T, 256, 2>::run(a, grid, flags, s);
-  if (a.cols <= 8192) return Launch<T, 512, 2>::run(a, grid, flags, s);
-  return Launch<T, 1024, 2>::run(a, grid, flags, s);
-}
-
-template <typename T, int G, int V>
-struct LaunchNorm {
-  static cudaError_t run(const NormArgs& a, int grid, unsigned int flags, cudaStream_t s) {
-    return launch(norm_kernel<T, G, V>, dim3(grid), G * kRowsPerBlock<G>, a, flags, s);
-  }
-};
-
-template <typename T, int G, int V>
-struct LaunchNormBackward {
-  static cudaError_t run(const NormBackwardArgs& a, int grid, unsigned int flags, cudaStream_t s) {
-    return launch(norm_backward_kernel<T, G, V>, dim3(grid), G * kRowsPerBlock<G>, a, flags, s);
-  }
-};
-
-int rows_per_block(int cols) { return cols <= 512 ? 4 : 1; }
-
-// Threads of the register kernels' blocks.
-int block_threads(int cols) {
-  return cols <= 2048 ? 128 : cols <= 4096 ? 256 : cols <= 8192 ? 512 : 1024;
-}
-
-// Blocks of the backward register kernel: as many as fill the SMs (about
-// 1024 threads of it each at its register use), at most one per row group.
-int64_t backward_blocks(int64_t rows, int64_t cols, int sm_count) {
-  const int64_t groups = (rows + rows_per_block(static_cast<int>(cols)) - 1) / rows_per_block(static_cast<int>(cols));
-  return std::max<int64_t>(1, std::min<int64_t>(groups, int64_t{sm_count} * (1024 / block_threads(static_cast<int>(cols)))));
-}
-
 int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
 
-// Row strips of the column kernels: enough blocks for four per SM.
+// Largest of 16, 8, 4, 2 that every row's start is a multiple of.
+int row_align(const void* p, int64_t ld) {
+  const uintptr_t both = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(ld * 2);
+  return both % 16 == 0 ? 16 : both % 8 == 0 ? 8 : both % 4 == 0 ? 4 : 2;
+}
+
+// Threads per row and vectors per thread of the register kernels: four
+// vectors, a warp at least.
+int group_threads(int64_t cols) {
+  return cols <= 1024 ? 32 : cols <= 2048 ? 64 : cols <= 4096 ? 128 : cols <= 8192 ? 256 : 512;
+}
+
+template <typename T, int G, int V>
+cudaError_t launch_rows(const NormArgs& a, int grid, unsigned int flags, cudaStream_t s) {
+  constexpr int kThreads = G < kNormThreads ? kNormThreads : G;
+  return a.vec ? launch(norm_kernel<T, G, V, true>, dim3(grid), kThreads, 0, a, flags, s)
+               : launch(norm_kernel<T, G, V, false>, dim3(grid), kThreads, 0, a, flags, s);
+}
+
+template <typename T>
+cudaError_t norm_by_columns(const NormArgs& a, int grid, unsigned int flags, cudaStream_t s) {
+  if (a.cols <= 256) return launch_rows<T, 32, 1>(a, grid, flags, s);
+  if (a.cols <= 512) return launch_rows<T, 32, 2>(a, grid, flags, s);
+  switch (group_threads(a.cols)) {
+    case 32: return launch_rows<T, 32, 4>(a, grid, flags, s);
+    case 64: return launch_rows<T, 64, 4>(a, grid, flags, s);
+    case 128: return launch_rows<T, 128, 4>(a, grid, flags, s);
+    case 256: return launch_rows<T, 256, 4>(a, grid, flags, s);
+    default: return launch_rows<T, 512, 4>(a, grid, flags, s);
+  }
+}
+
+template <typename T, int G, int V>
+cudaError_t launch_rows_backward(const NormBackwardArgs& a, int grid, unsigned int flags, cudaStream_t s) {
+  constexpr int kGroups = kRowThreads / G;
+  // Weight and rings (at most 224 KB), then the groups' sums (at most 128 KB).
+  const size_t one = static_cast<size_t>(a.part_cols) * sizeof(float);
+  const size_t ring = a.vec ? static_cast<size_t>(kGroups) * kBackwardStages<G> * 2 * a.cols * 2 : 0;
+  const size_t smem = std::max(one + ring, kGroups > 1 ? kGroups * 2 * one : 0);
+  return a.vec ? launch(norm_backward_kernel<T, G, V, true>, dim3(grid), kRowThreads, smem, a, flags, s)
+               : launch(norm_backward_kernel<T, G, V, false>, dim3(grid), kRowThreads, smem, a, flags, s);
+}
+
+template <typename T>
+cudaError_t norm_backward_by_columns(const NormBackwardArgs& a, int grid, unsigned int flags, cudaStream_t s) {
+  if (a.cols <= 256) return launch_rows_backward<T, 32, 1>(a, grid, flags, s);
+  if (a.cols <= 512) return launch_rows_backward<T, 32, 2>(a, grid, flags, s);
+  switch (group_threads(a.cols)) {
+    case 32: return launch_rows_backward<T, 32, 4>(a, grid, flags, s);
+    case 64: return launch_rows_backward<T, 64, 4>(a, grid, flags, s);
+    case 128: return launch_rows_backward<T, 128, 4>(a, grid, flags, s);
+    case 256: return launch_rows_backward<T, 256, 4>(a, grid, flags, s);
+    default: return launch_rows_backward<T, 512, 4>(a, grid, flags, s);
+  }
+}
+
+// Blocks of the backward register kernel: one per SM, at most one per rows
+// that a block takes at a time.
+int64_t backward_blocks(int64_t rows, int64_t cols, int sm_count) {
+  const int64_t at_a_time = kRowThreads / group_threads(cols);
+  return std::min<int64_t>((rows + at_a_time - 1) / at_a_time, sm_count);
+}
+
+template <typename T, int G, int V>
+cudaError_t set_attr() {
+  constexpr cudaFuncAttribute kAttr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  const cudaError_t e = cudaFuncSetAttribute(norm_backward_kernel<T, G, V, true>, kAttr, 229376);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(norm_backward_kernel<T, G, V, false>, kAttr, 131072);
+}
+
+template <typename T>
+cudaError_t set_attrs() {
+  cudaError_t e = set_attr<T, 32, 1>();
+  if (e == cudaSuccess) e = set_attr<T, 32, 2>();
+  if (e == cudaSuccess) e = set_attr<T, 32, 4>();
+  if (e == cudaSuccess) e = set_attr<T, 64, 4>();
+  if (e == cudaSuccess) e = set_attr<T, 128, 4>();
+  if (e == cudaSuccess) e = set_attr<T, 256, 4>();
+  if (e == cudaSuccess) e = set_attr<T, 512, 4>();
+  return e;
+}
+
+// Row strips of the column kernels: four blocks of 128 threads per SM.
 int64_t strips(int64_t rows, int64_t cols, int sm_count) {
   const int64_t across = (cols + 1023) / 1024;
-  return std::max<int64_t>(1, std::min<int64_t>(rows, std::min<int64_t>(4096, (int64_t{sm_count} * 8 + across - 1) / across)));
+  return std::max<int64_t>(1, std::min<int64_t>(rows, std::min<int64_t>(4096, (int64_t{sm_count} * 4 + across - 1) / across)));
 }
 
 template <typename T>
 cudaError_t norm_typed(const NormArgs& a, int sm_count, unsigned int flags, cudaStream_t s) {
   if (a.cols > kNormRegisterCols) {
-    return launch(norm_long_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(a.rows, 2 * sm_count))), 1024, a,
+    return launch(norm_long_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(a.rows, 2 * sm_count))), 1024, 0, a,
                   flags, s);
   }
-  const int64_t groups = (a.rows + rows_per_block(a.cols) - 1) / rows_per_block(a.cols);
-  return by_columns<T, LaunchNorm>(a, static_cast<int>(std::min<int64_t>(groups, 1 << 20)), flags, s);
+  // As many blocks as an SM holds: three of 256 threads, one of 512.
+  const int g = group_threads(a.cols);
+  const int64_t at_a_time = g < kNormThreads ? kNormThreads / g : 1;
+  const int64_t blocks =
+      std::min<int64_t>((a.rows + at_a_time - 1) / at_a_time, int64_t{sm_count} * (g < 512 ? 3 : 1));
+  return norm_by_columns<T>(a, static_cast<int>(blocks), flags, s);
 }
 
 template <typename T>
@@ -522,16 +826,16 @@ cudaError_t norm_backward_typed(NormBackwardArgs a, void* dweight, void* dbias, 
   cudaError_t e;
   if (a.cols > kNormRegisterCols) {
     e = launch(norm_backward_long_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(a.rows, 2 * sm_count))),
-               1024, a, flags, s);
+               1024, 0, a, flags, s);
     parts = strips(a.rows, a.cols, sm_count);
     if (e == cudaSuccess && a.part != nullptr) {
       e = launch(norm_columns_kernel<T>, dim3(static_cast<unsigned>((a.cols + 1023) / 1024), static_cast<unsigned>(parts)),
-                 128, a, flags, s);
+                 128, 0, a, flags, s);
     }
   } else {
     const int64_t grid = backward_blocks(a.rows, a.cols, sm_count);
-    parts = grid * rows_per_block(a.cols);
-    e = by_columns<T, LaunchNormBackward>(a, static_cast<int>(grid), flags, s);
+    parts = grid;
+    e = norm_backward_by_columns<T>(a, static_cast<int>(grid), flags, s);
   }
   if (e != cudaSuccess || a.part == nullptr) return e;
   ColumnSumArgs c = {};
@@ -542,15 +846,15 @@ cudaError_t norm_backward_typed(NormBackwardArgs a, void* dweight, void* dbias, 
   c.cols = a.cols;
   c.out[0] = dweight;
   c.out[1] = dbias;
-  return launch(column_sum_kernel<T>, dim3(static_cast<unsigned>((a.cols + 31) / 32), 2), 256, c, flags, s);
+  return launch(column_sum_kernel<T>, dim3(static_cast<unsigned>((a.cols + 31) / 32), 2), 32 * kSumRanges, 0, c, flags, s);
 }
 
 template <typename T>
 cudaError_t act_backward_typed(const ActBackwardArgs& a, bool gated, void* const* dbias, int64_t n_strips,
                                unsigned int flags, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>((a.cols + 1023) / 1024), static_cast<unsigned>(n_strips));
-  cudaError_t e = gated ? launch(act_backward_kernel<T, true>, grid, 128, a, flags, s)
-                        : launch(act_backward_kernel<T, false>, grid, 128, a, flags, s);
+  cudaError_t e = gated ? launch(act_backward_kernel<T, true>, grid, 128, 0, a, flags, s)
+                        : launch(act_backward_kernel<T, false>, grid, 128, 0, a, flags, s);
   if (e != cudaSuccess || a.part == nullptr) return e;
   ColumnSumArgs c = {};
   c.part = a.part;
@@ -560,17 +864,22 @@ cudaError_t act_backward_typed(const ActBackwardArgs& a, bool gated, void* const
   c.cols = a.cols;
   c.out[0] = dbias[0];
   c.out[1] = gated ? dbias[1] : nullptr;
-  return launch(column_sum_kernel<T>, dim3(static_cast<unsigned>((a.cols + 31) / 32), static_cast<unsigned>(c.sums)), 256,
-                c, flags, s);
+  return launch(column_sum_kernel<T>, dim3(static_cast<unsigned>((a.cols + 31) / 32), static_cast<unsigned>(c.sums)),
+                32 * kSumRanges, 0, c, flags, s);
 }
 
 }  // namespace
+
+cudaError_t rows_prepare_device() {
+  const cudaError_t e = set_attrs<__half>();
+  return e != cudaSuccess ? e : set_attrs<__nv_bfloat16>();
+}
 
 size_t norm_backward_partial_bytes(int64_t rows, int64_t cols, int sm_count) {
   if (rows <= 0 || cols <= 0) return 0;
   const int64_t parts = cols > kNormRegisterCols
                             ? strips(rows, cols, sm_count)
-                            : backward_blocks(rows, cols, sm_count) * rows_per_block(static_cast<int>(cols));
+                            : backward_blocks(rows, cols, sm_count);
   return static_cast<size_t>(parts * 2 * padded(cols)) * sizeof(float);
 }
 
@@ -580,16 +889,18 @@ size_t act_backward_partial_bytes(int64_t rows, int64_t cols, int sums, int sm_c
 }
 
 cudaError_t launch_norm(int dtype, NormArgs a, int sm_count, unsigned int flags, cudaStream_t s) {
-  a.vec = vec_rows(a.x, a.ld_x, a.cols) && vec_rows(a.y, a.ld_y, a.cols);
-  a.vec_w = vec_rows(a.weight, 0, a.cols) && vec_rows(a.bias, 0, a.cols);
+  a.align = std::min(row_align(a.x, a.ld_x), row_align(a.y, a.ld_y));
+  a.align_w = std::min(row_align(a.weight, 0), row_align(a.bias, 0));
+  a.vec = a.align == 16 && a.align_w == 16 && a.cols % 8 == 0;
   return dtype == GLQ_DTYPE_BF16 ? norm_typed<__nv_bfloat16>(a, sm_count, flags, s)
                                  : norm_typed<__half>(a, sm_count, flags, s);
 }
 
 cudaError_t launch_norm_backward(int dtype, NormBackwardArgs a, void* dweight, void* dbias, int sm_count,
                                  unsigned int flags, cudaStream_t s) {
-  a.vec = vec_rows(a.x, a.ld_x, a.cols) && vec_rows(a.dy, a.ld_dy, a.cols) && vec_rows(a.dx, a.ld_dx, a.cols);
-  a.vec_w = vec_rows(a.weight, 0, a.cols);
+  a.align = std::min(row_align(a.x, a.ld_x), std::min(row_align(a.dy, a.ld_dy), row_align(a.dx, a.ld_dx)));
+  a.align_w = row_align(a.weight, 0);
+  a.vec = a.align == 16 && a.cols % 8 == 0;
   a.part_cols = padded(a.cols);
   return dtype == GLQ_DTYPE_BF16 ? norm_backward_typed<__nv_bfloat16>(a, dweight, dbias, sm_count, flags, s)
                                  : norm_backward_typed<__half>(a, dweight, dbias, sm_count, flags, s);
@@ -597,9 +908,9 @@ cudaError_t launch_norm_backward(int dtype, NormBackwardArgs a, void* dweight, v
 
 cudaError_t launch_act_backward(int dtype, bool gated, ActBackwardArgs a, void* const* dbias, int sm_count,
                                 unsigned int flags, cudaStream_t s) {
-  a.vec_dy = vec_rows(a.dy, a.ld_dy, a.cols);
-  a.vec_pre = vec_rows(a.pre[0], a.ld_pre, a.cols) && vec_rows(a.pre[1], a.ld_pre, a.cols);
-  a.vec_dz = vec_rows(a.dz[0], a.ld_dz, a.cols) && vec_rows(a.dz[1], a.ld_dz, a.cols);
+  a.align_dy = row_align(a.dy, a.ld_dy);
+  a.align_pre = std::min(row_align(a.pre[0], a.ld_pre), row_align(a.pre[1], a.ld_pre));
+  a.align_dz = std::min(row_align(a.dz[0], a.ld_dz), row_align(a.dz[1], a.ld_dz));
   a.part_cols = padded(a.cols);
   const int64_t n = strips(a.rows, a.cols, sm_count);
   return dtype == GLQ_DTYPE_BF16 ? act_backward_typed<__nv_bfloat16>(a, gated, dbias, n, flags, s)

@@ -12,7 +12,7 @@ namespace glq {
 constexpr int kNormRegisterCols = 16384;
 
 // Tensors are [rows, cols] with unit column stride and row pitch ld_*
-// (elements); the vec_* fields are set by the launchers.
+// (elements); the align and vec fields are set by the launchers.
 struct NormArgs {
   const void* x;
   long long ld_x;
@@ -25,7 +25,9 @@ struct NormArgs {
   long long rows;
   int cols;
   float eps;
-  int vec, vec_w;
+  unsigned int* err;
+  int align, align_w;  // bytes that rows, weight and bias start at multiples of
+  int vec;             // rows of whole 16-byte vectors
 };
 
 struct NormBackwardArgs {
@@ -42,7 +44,8 @@ struct NormBackwardArgs {
   long long part_cols;
   long long rows;
   int cols;
-  int vec, vec_w;
+  unsigned int* err;
+  int align, align_w, vec;
 };
 
 struct ColumnSumArgs {
@@ -64,8 +67,11 @@ struct ActBackwardArgs {
   long long rows;
   int cols;
   int act;
-  int vec_dy, vec_pre, vec_dz;
+  int align_dy, align_pre, align_dz;
 };
+
+// Per-device one-time set-up (shared memory opt-in).
+cudaError_t rows_prepare_device();
 
 size_t norm_backward_partial_bytes(int64_t rows, int64_t cols, int sm_count);
 size_t act_backward_partial_bytes(int64_t rows, int64_t cols, int sums, int sm_count);
