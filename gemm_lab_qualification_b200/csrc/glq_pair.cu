@@ -19,6 +19,11 @@
 //   * Persistent grid; warp 0 feeds a TMA ring, warp 1 of the leader issues
 //     tcgen05.mma, warps 4-7 run the epilogue of one tile from tensor memory
 //     while the next tile accumulates in the other half of it.
+//   * Few tiles (a wave that would leave SMs idle): the K range of a tile is
+//     split over the pairs of one larger cluster (SPLIT).  Each CTA leaves its
+//     FP32 partial tile in its drained ring; after a cluster barrier the pairs
+//     share out the tile's column chunks, read the partials through
+//     distributed shared memory and add them in split order.
 //   * Operands are K-major or MN-major (the transposed operands of the
 //     backward products), both read by TMA as they lie in memory: no
 //     transposition pass.
@@ -51,6 +56,7 @@ constexpr int kSlots = 4;       // staging buffers per epilogue warp
 constexpr uint32_t kSlotBytes = 32 * 128;  // 32 rows x 64 16-bit columns
 constexpr uint32_t kMnBox = 64 * kBK * 2;  // MN-major box: 64 elements x 64 K rows
 constexpr uint32_t kSmemMax = 232448;
+constexpr int kMaxPairs = 4;  // K ranges of a split tile: clusters of up to 8 CTAs
 
 template <int BN>
 struct PairConfig {
@@ -66,6 +72,7 @@ struct PairConfig {
   static constexpr int kBars = 2 * kStages + 4;
   static constexpr uint32_t kSmem = 1024 + kRing + kStaging + kBias + kBars * 8 + 16;
   static constexpr uint32_t kTmemCols = 2 * BN;  // two accumulators
+  static_assert(128 * BN * 4 <= kRing, "a split tile's partials reuse the ring");
   static_assert(kSmem <= kSmemMax, "shared memory");
 };
 
@@ -79,6 +86,7 @@ struct PairArgs {
   int outputs;           // 2: Parts::kTwo
   int kb_part, kb_total; // K blocks of the first contraction range, of all
   int group_m;           // tile rows that share a column of tiles in launch order
+  int split;             // K ranges per tile (SPLIT kernels), pairs per cluster
   int act;
   const void* bias[2];
   const void* residual;
@@ -115,7 +123,7 @@ __device__ __forceinline__ Tile tile_at(const PairArgs& args, int t) {
   return c;
 }
 
-template <typename T, bool A_MN, bool B_MN, int BN, bool GATED>
+template <typename T, bool A_MN, bool B_MN, int BN, bool GATED, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ PairArgs args) {
   using Cfg = PairConfig<BN>;
@@ -142,10 +150,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = ptx::cluster_ctarank();
+  const uint32_t cluster_rank = ptx::cluster_ctarank();
+  const uint32_t rank = cluster_rank & 1u;                // half of the pair
+  const uint32_t leader = cluster_rank & ~1u;             // the pair's CTA that issues the MMAs
+  const int range = static_cast<int>(cluster_rank >> 1);  // K range of this pair (SPLIT)
   const int num_tiles = args.outputs * args.tiles_m * args.tiles_n;
-  const int first_tile = static_cast<int>(blockIdx.x >> 1);
-  const int tile_step = static_cast<int>(gridDim.x >> 1);
+  const int split = SPLIT ? args.split : 1;
+  const int first_tile = static_cast<int>(blockIdx.x >> 1) / split;
+  // A SPLIT cluster computes one tile.
+  const int tile_step = SPLIT ? num_tiles : static_cast<int>(gridDim.x >> 1);
+  const int kb_begin = SPLIT ? static_cast<int>(static_cast<long long>(range) * args.kb_total / split) : 0;
+  const int kb_end = SPLIT ? static_cast<int>(static_cast<long long>(range + 1) * args.kb_total / split) : args.kb_total;
   auto raise = [&](unsigned int bit) {
     atomicOr(args.err, bit);
     *abort_flag = 1;
@@ -186,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Tile tile = tile_at<kTileN>(args, t);
       const int a_row = tile.m0 + static_cast<int>(rank) * 128;
       const int b_row = GATED ? tile.n0 : tile.n0 + static_cast<int>(rank) * (BN / 2);
-      for (int kb = 0; kb < args.kb_total; ++kb, ++it) {
+      for (int kb = kb_begin; kb < kb_end; ++kb, ++it) {
         const int stage = it % kStages;
         const int round = it / kStages;
         if (round > 0 &&
@@ -201,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t a_dst = sbase + stage * Cfg::kStageBytes;
         const uint32_t b_dst = a_dst + Cfg::kABytes;
         if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * Cfg::kStageBytes);
-        const uint32_t signal = ptx::map_to_rank(full_bar(stage), 0);
+        const uint32_t signal = ptx::map_to_rank(full_bar(stage), leader);
         if constexpr (A_MN) {
           ptx::tma_load_2d_pair(a_dst, map_a, a_row, k0, signal);
           ptx::tma_load_2d_pair(a_dst + kMnBox, map_a, a_row + 64, k0, signal);
@@ -231,6 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // K-major row, or 16 K rows of 128 bytes.
     constexpr uint32_t kAStep = A_MN ? 128 : 2;
     constexpr uint32_t kBStep = B_MN ? 128 : 2;
+    const uint16_t pair_mask = static_cast<uint16_t>(3u << leader);
     int it = 0, local = 0;
     for (int t = first_tile; t < num_tiles && *abort_flag == 0; t += tile_step, ++local) {
       const int acc = local & 1;
@@ -242,9 +258,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::tc_fence_after_sync();
       const uint32_t d = tmem + acc * BN;
       bool ok = true;
-      for (int kb = 0; kb < args.kb_total; ++kb, ++it) {
+      for (int kb = kb_begin; kb < kb_end; ++kb, ++it) {
         const int stage = it % kStages;
-        if (!ptx::mbar_wait_bounded_cluster(full_bar(stage), (it / kStages) & 1, abort_flag, kWaitBudgetNs)) {
+        if (!ptx::mbar_wait_bounded(full_bar(stage), (it / kStages) & 1, abort_flag, kWaitBudgetNs)) {
           raise(kErrTimeoutMma);
           ok = false;
           break;
@@ -256,12 +272,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t db = B_MN ? ptx::umma_desc_mn_sw128(b_src) : ptx::umma_desc_k_sw128(b_src);
 #pragma unroll
         for (int kk = 0; kk < kBK / 16; ++kk) {
-          ptx::tc_mma_f16_pair(d, da + kAStep * kk, db + kBStep * kk, idesc, kb > 0 || kk > 0 ? 1u : 0u);
+          ptx::tc_mma_f16_pair(d, da + kAStep * kk, db + kBStep * kk, idesc, kb > kb_begin || kk > 0 ? 1u : 0u);
         }
-        ptx::tc_commit_pair(empty_bar(stage));
+        ptx::tc_commit_pair(empty_bar(stage), pair_mask);
       }
       if (!ok) break;
-      ptx::tc_commit_pair(acc_full(acc));
+      ptx::tc_commit_pair(acc_full(acc), pair_mask);
     }
   } else if (warp >= 4) {
     // ---- Epilogue: warp w holds tile rows 32 (w % 4) .. + 31, lane = row.
@@ -274,10 +290,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Staging buffers a column chunk fills: the output and what is kept.
     const int per_chunk = 1 + (keep ? (GATED ? 2 : 1) : 0);
     int slot = 0, local = 0;
+    bool joined = false;
     for (int t = first_tile; t < num_tiles; t += tile_step, ++local) {
       const int acc = local & 1;
       const bool ready =
-          ptx::mbar_wait_bounded_cluster(acc_full(acc), (local >> 1) & 1, abort_flag, kWaitBudgetNs);
+          ptx::mbar_wait_bounded(acc_full(acc), (local >> 1) & 1, abort_flag, kWaitBudgetNs);
       if (!__all_sync(0xffffffffu, ready)) {  // the warp leaves together
         if (lane == 0) raise(kErrTimeoutEpilogue);
         break;
@@ -287,8 +304,56 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row0 = tile.m0 + static_cast<int>(rank) * 128 + w * 32;
       const int row = row0 + lane;
       const uint32_t src = lane_base + acc * BN;
+      if constexpr (SPLIT) {
+        // FP32 partials into the drained ring: [group of 4 columns][tile row].
+        float4* part = reinterpret_cast<float4*>(smem) + w * 32 + lane;
 #pragma unroll 1
-      for (int c = 0; c < kTileN; c += 64) {
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t r[32];
+          ptx::tmem_ld_32x32b_x32(src + c, r);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            part[(c / 4 + q) * 128] = make_float4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]),
+                                                  __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]));
+          }
+        }
+        joined = true;
+        ptx::cluster_arrive_release();
+        ptx::cluster_wait();
+      }
+      // 32 accumulator columns from `at`: from tensor memory, or the sums of
+      // the cluster's partials in split order.
+      auto load32 = [&](int at, uint32_t(&r)[32]) {
+        if constexpr (SPLIT) {
+          const uint32_t local_at = sbase + static_cast<uint32_t>((at / 4 * 128 + w * 32 + lane) * 16);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            float4 x[kMaxPairs];
+#pragma unroll
+            for (int p = 0; p < kMaxPairs; ++p) {
+              if (p < split) x[p] = ptx::ld_dsmem_v4(ptx::map_to_rank(local_at + q * 128 * 16, 2 * p + rank));
+            }
+#pragma unroll
+            for (int p = 1; p < kMaxPairs; ++p) {
+              if (p < split) {
+                x[0].x += x[p].x;
+                x[0].y += x[p].y;
+                x[0].z += x[p].z;
+                x[0].w += x[p].w;
+              }
+            }
+            r[4 * q] = __float_as_uint(x[0].x);
+            r[4 * q + 1] = __float_as_uint(x[0].y);
+            r[4 * q + 2] = __float_as_uint(x[0].z);
+            r[4 * q + 3] = __float_as_uint(x[0].w);
+          }
+        } else {
+          ptx::tmem_ld_32x32b_x32(src + at, r);
+        }
+      };
+#pragma unroll 1
+      for (int c = SPLIT ? 64 * range : 0; c < kTileN; c += SPLIT ? 64 * split : 64) {
         const int col0 = tile.n0 + c;
         // The buffers about to be filled must have been read by their stores.
         if (lane == 0) {
@@ -308,9 +373,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int h = 0; h < 2; ++h) {
           const int u0 = col0 + 32 * h;  // first output column of this unit
           uint32_t r[32];
-          ptx::tmem_ld_32x32b_x32(src + c + 32 * h, r);
+          load32(c + 32 * h, r);
           [[maybe_unused]] uint32_t r2[32];
-          if constexpr (GATED) ptx::tmem_ld_32x32b_x32(src + BN / 2 + c + 32 * h, r2);
+          if constexpr (GATED) load32(BN / 2 + c + 32 * h, r2);
           __syncwarp();
           {
             const bool in = u0 + lane < args.n;
@@ -322,12 +387,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           __syncwarp();
-          ptx::tmem_ld_wait();
-          if (c + 64 >= kTileN && h == 1) {
+          if constexpr (!SPLIT) ptx::tmem_ld_wait();
+          if (!SPLIT && c + 64 >= kTileN && h == 1) {
             // The accumulator is in registers: the leader may reuse it.
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(acc_empty(acc), 0));
+            if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(acc_empty(acc), leader));
           }
           float v[32];
 #pragma unroll
@@ -429,8 +494,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (lane == 0) ptx::bulk_wait_all();
+    // An aborted epilogue still takes its part in the join's barrier.
+    if (SPLIT && !joined) {
+      ptx::cluster_arrive_release();
+      ptx::cluster_wait();
+    }
   }
   __syncwarp();
+  if (SPLIT && warp < 4) {
+    ptx::cluster_arrive_release();
+    ptx::cluster_wait();
+  }
   ptx::tc_fence_before_sync();
   __syncthreads();
   ptx::cluster_sync();  // the peer's MMA operands and barriers are no longer needed
@@ -451,8 +525,14 @@ bool operand_map(CUtensorMap* map, int dtype, const Operand& o, int64_t rows, in
                    : encode_tile_map(map, dtype, o.base, k, rows, o.pitch, kBK);
 }
 
-template <typename T, bool A_MN, bool B_MN, int BN, bool GATED>
-cudaError_t launch_typed(const Product& p, int sm_count, unsigned int* err, cudaStream_t s) {
+// How a product is cut up: columns per tile and K ranges per tile.
+struct Cut {
+  int bn;
+  int split;
+};
+
+template <typename T, bool A_MN, bool B_MN, int BN, bool GATED, bool SPLIT>
+cudaError_t launch_typed(const Product& p, int split, int sm_count, unsigned int* err, cudaStream_t s) {
   using Cfg = PairConfig<BN>;
   constexpr int kTileN = GATED ? BN / 2 : BN;
   const bool concat = p.parts == Parts::kConcatK, two = p.parts == Parts::kTwo;
@@ -491,6 +571,7 @@ cudaError_t launch_typed(const Product& p, int sm_count, unsigned int* err, cuda
   args.kb_part = static_cast<int>((p.k + kBK - 1) / kBK);
   args.kb_total = args.kb_part * (concat ? 2 : 1);
   args.group_m = 16;
+  args.split = split;
   args.act = p.act;
   args.residual = p.residual;
   args.ld_residual = p.ld_residual;
@@ -499,43 +580,58 @@ cudaError_t launch_typed(const Product& p, int sm_count, unsigned int* err, cuda
   args.ld_pre = p.ld_pre;
   args.err = err;
   const int64_t tiles = static_cast<int64_t>(args.outputs) * args.tiles_m * args.tiles_n;
+  const int64_t pairs = SPLIT ? tiles * split : std::min<int64_t>(tiles, std::max(sm_count / 2, 1));
 
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(tiles, std::max(sm_count / 2, 1))));
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Cfg::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.x = SPLIT ? 2 * split : 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (p.flags & GLQ_FLAG_NO_PDL) ? 1 : 2;
-  return cudaLaunchKernelEx(&cfg, pair_kernel<T, A_MN, B_MN, BN, GATED>, maps, args);
+  return cudaLaunchKernelEx(&cfg, pair_kernel<T, A_MN, B_MN, BN, GATED, SPLIT>, maps, args);
 }
 
-// The operand orders that occur: both K-major or B MN-major (forward and
-// input gradient), both MN-major (weight gradient).
-template <typename T, int BN>
-cudaError_t launch_order(const Product& p, int sm_count, unsigned int* err, cudaStream_t s) {
+template <typename T, int BN, bool SPLIT>
+cudaError_t launch_order(const Product& p, int split, int sm_count, unsigned int* err, cudaStream_t s) {
+  // The operand orders that occur: both K-major or B MN-major (forward and
+  // input gradient), both MN-major (weight gradient).
   const bool a_mn = !p.a[0].k_major, b_mn = !p.b[0].k_major;
   if (p.parts == Parts::kGated) {
     if (a_mn) return cudaErrorInvalidValue;
-    return b_mn ? launch_typed<T, false, true, BN, true>(p, sm_count, err, s)
-                : launch_typed<T, false, false, BN, true>(p, sm_count, err, s);
+    return b_mn ? launch_typed<T, false, true, BN, true, SPLIT>(p, split, sm_count, err, s)
+                : launch_typed<T, false, false, BN, true, SPLIT>(p, split, sm_count, err, s);
   }
-  if (a_mn) return b_mn ? launch_typed<T, true, true, BN, false>(p, sm_count, err, s) : cudaErrorInvalidValue;
-  return b_mn ? launch_typed<T, false, true, BN, false>(p, sm_count, err, s)
-              : launch_typed<T, false, false, BN, false>(p, sm_count, err, s);
+  if (a_mn) {
+    return b_mn ? launch_typed<T, true, true, BN, false, SPLIT>(p, split, sm_count, err, s) : cudaErrorInvalidValue;
+  }
+  return b_mn ? launch_typed<T, false, true, BN, false, SPLIT>(p, split, sm_count, err, s)
+              : launch_typed<T, false, false, BN, false, SPLIT>(p, split, sm_count, err, s);
+}
+
+template <typename T>
+cudaError_t launch_cut(const Product& p, Cut cut, int sm_count, unsigned int* err, cudaStream_t s) {
+  if (cut.split > 1) {
+    return cut.bn == 256 ? launch_order<T, 256, true>(p, cut.split, sm_count, err, s)
+                         : launch_order<T, 128, true>(p, cut.split, sm_count, err, s);
+  }
+  return cut.bn == 256 ? launch_order<T, 256, false>(p, 1, sm_count, err, s)
+                       : launch_order<T, 128, false>(p, 1, sm_count, err, s);
 }
 
 template <typename T, bool A_MN, bool B_MN, int BN, bool GATED>
 cudaError_t set_attr() {
-  return cudaFuncSetAttribute(pair_kernel<T, A_MN, B_MN, BN, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(PairConfig<BN>::kSmem));
+  constexpr cudaFuncAttribute kAttr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  const int bytes = static_cast<int>(PairConfig<BN>::kSmem);
+  const cudaError_t e = cudaFuncSetAttribute(pair_kernel<T, A_MN, B_MN, BN, GATED, false>, kAttr, bytes);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(pair_kernel<T, A_MN, B_MN, BN, GATED, true>, kAttr, bytes);
 }
 
 template <typename T, int BN>
@@ -548,18 +644,54 @@ cudaError_t set_attrs() {
   return e;
 }
 
+// Clusters of 2 * split CTAs that run at once, one CTA per SM (148 SMs in
+// GPCs of 16 to 20).
+int resident_clusters(int split, int sm_count) {
+  return split == 1 ? sm_count / 2 : split == 2 ? sm_count * 33 / 148 : split == 3 ? sm_count * 20 / 148 : sm_count * 16 / 148;
+}
+
+// The cut with the least estimated time: waves of tiles times (K blocks per
+// range at the tile's rate, plus what a tile costs outside its main loop).
+Cut choose_cut(const Product& p, int sm_count) {
+  const bool gated = p.parts == Parts::kGated;
+  const int64_t kb = (p.k + kBK - 1) / kBK * (p.parts == Parts::kConcatK ? 2 : 1);
+  Cut best = {256, 1};
+  double best_us = 0.0;
+  for (int bn = 256; bn >= 128; bn /= 2) {
+    const int tile_n = gated ? bn / 2 : bn;
+    const int64_t tiles =
+        (p.m + kTileM - 1) / kTileM * ((p.n + tile_n - 1) / tile_n) * (p.parts == Parts::kTwo ? 2 : 1);
+    for (int split = 1; split <= kMaxPairs && split <= kb; ++split) {
+      const int64_t at_once = std::max(resident_clusters(split, sm_count), 1);
+      const int64_t waves = (tiles + at_once - 1) / at_once;
+      const double block_us = bn == 256 ? 0.40 : 0.23;
+      const double tail_us = (bn == 256 ? 2.0 : 1.0) + (split > 1 ? 2.0 : 0.0);
+      const double us = static_cast<double>(waves) * static_cast<double>((kb + split - 1) / split) * block_us +
+                        (split > 1 ? static_cast<double>(waves) : 1.0) * tail_us;
+      if (best_us == 0.0 || us < best_us) {
+        best_us = us;
+        best = {bn, split};
+      }
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 cudaError_t pair_prepare_device() {
   cudaError_t e = set_attrs<__half, 256>();
+  if (e == cudaSuccess) e = set_attrs<__half, 128>();
   if (e == cudaSuccess) e = set_attrs<__nv_bfloat16, 256>();
+  if (e == cudaSuccess) e = set_attrs<__nv_bfloat16, 128>();
   return e;
 }
 
 cudaError_t launch_pair(const Product& p, int sm_count, unsigned int* err, cudaStream_t s) {
   if (p.m < 1 || p.n < 1 || p.k < 1) return cudaErrorInvalidValue;
-  return p.dtype == GLQ_DTYPE_BF16 ? launch_order<__nv_bfloat16, 256>(p, sm_count, err, s)
-                                   : launch_order<__half, 256>(p, sm_count, err, s);
+  Cut cut = choose_cut(p, sm_count);
+  return p.dtype == GLQ_DTYPE_BF16 ? launch_cut<__nv_bfloat16>(p, cut, sm_count, err, s)
+                                   : launch_cut<__half>(p, cut, sm_count, err, s);
 }
 
 }  // namespace glq

@@ -65,12 +65,13 @@ __device__ __forceinline__ void tc_mma_f16_pair(uint32_t d_tmem, uint64_t a_desc
       : "memory");
 }
 
-// Arrives once on the barrier at this offset in both CTAs when every pair
-// MMA this thread issued before has completed.
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+// Arrives once on the barrier at this offset in the CTAs of `cta_mask` (the
+// pair's two cluster ranks) when every pair MMA this thread issued before has
+// completed.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar, uint16_t cta_mask) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"(static_cast<uint16_t>(3))
+      "h"(cta_mask)
       : "memory");
 }
 
