@@ -64,8 +64,9 @@ cudaError_t pair_prepare_device();
 cudaError_t skinny_prepare_device();
 
 // Tensor map of a row-major matrix rows x cols (row pitch in elements of two
-// bytes), boxes of box_rows x 64 columns, 128-byte swizzle, zero fill.
+// bytes), boxes of box_rows x box_cols (64 columns with 128-byte swizzle, or 32
+// with 64-byte swizzle), zero fill.
 bool encode_tile_map(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t cols, int64_t pitch,
-                     uint32_t box_rows);
+                     uint32_t box_rows, uint32_t box_cols = 64);
 
 }  // namespace glq

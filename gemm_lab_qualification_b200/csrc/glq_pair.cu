@@ -17,8 +17,11 @@
 //     [0, BN / 2) of every accumulator row are gate and [BN / 2, BN) are up,
 //     in the same TMEM lane: the product needs no exchange.
 //   * Persistent grid; warp 0 feeds a TMA ring, warp 1 of the leader issues
-//     tcgen05.mma, warps 4-7 run the epilogue of one tile from tensor memory
-//     while the next tile accumulates in the other half of it.
+//     tcgen05.mma, warps 4-11 run the epilogue of one tile from tensor memory
+//     while the next tile accumulates in the other half of it.  Two epilogue
+//     warps per SM sub-partition: with one, nothing hid the latency of a chain
+//     of tensor-memory load, conversion and store, and a 128 x 256 tile took
+//     4.8 us, longer than the main loop of K = 1000.
 //   * Few tiles (a wave that would leave SMs idle): the K range of a tile is
 //     split over the pairs of one larger cluster (SPLIT).  Each CTA leaves its
 //     FP32 partial tile in its drained ring; after a cluster barrier the pairs
@@ -27,11 +30,11 @@
 //   * Operands are K-major or MN-major (the transposed operands of the
 //     backward products), both read by TMA as they lie in memory: no
 //     transposition pass.
-//   * The epilogue works on 32 accumulator columns at a time in FP32, rounds
-//     once to the 16-bit output, stages 32 rows x 64 columns per warp in
-//     128-byte-swizzled shared memory and lets the TMA store them (clipped at
-//     the edges), or, where the output's pitch or base is off 16 bytes, copies
-//     them out element by element.
+//   * The epilogue works on units of 32 rows x 32 accumulator columns per warp
+//     in FP32, rounds once to the 16-bit output, stages the unit in swizzled
+//     shared memory and lets the TMA store it (clipped at the edges), or, where
+//     the output's pitch or base is off 16 bytes, copies it out element by
+//     element.
 //
 // Every wait is bounded; an expired one raises a bit in the device error word
 // and the kernel returns.
@@ -49,11 +52,11 @@ namespace glq {
 namespace {
 
 constexpr int kBK = 64;         // K elements per stage: one 128-byte swizzle row
-constexpr int kThreads = 256;
+constexpr int kThreads = 384;
 constexpr int kTileM = 256;     // rows per pair
-constexpr int kEpiWarps = 4;    // warps 4..7, one per 32 TMEM lanes
+constexpr int kEpiWarps = 8;    // warps 4..11, two per 32 TMEM lanes
 constexpr int kSlots = 4;       // staging buffers per epilogue warp
-constexpr uint32_t kSlotBytes = 32 * 128;  // 32 rows x 64 16-bit columns
+constexpr uint32_t kSlotBytes = 32 * 64;  // a unit: 32 rows x 32 16-bit columns
 constexpr uint32_t kMnBox = 64 * kBK * 2;  // MN-major box: 64 elements x 64 K rows
 constexpr uint32_t kSmemMax = 232448;
 constexpr int kMaxPairs = 4;  // K ranges of a split tile: clusters of up to 8 CTAs
@@ -67,7 +70,7 @@ struct PairConfig {
   static constexpr uint32_t kStageBytes = kABytes + kBBytes;
   static constexpr uint32_t kRing = kStages * kStageBytes;
   static constexpr uint32_t kStaging = kEpiWarps * kSlots * kSlotBytes;
-  static constexpr uint32_t kBias = kEpiWarps * 64 * sizeof(float);
+  static constexpr uint32_t kBias = kEpiWarps * 64 * 2;  // a unit's columns of both biases
   // full, empty, accumulator full (2) and empty (2); TMEM slot, abort flag.
   static constexpr int kBars = 2 * kStages + 4;
   static constexpr uint32_t kSmem = 1024 + kRing + kStaging + kBias + kBars * 8 + 16;
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = smem_dyn + pad;
   const uint32_t sbase = raw + pad;
   uint8_t* staging = smem + Cfg::kRing;
-  float* bias_smem = reinterpret_cast<float*>(staging + Cfg::kStaging);
+  T* bias_smem = reinterpret_cast<T*>(staging + Cfg::kStaging);
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(bias_smem) + Cfg::kBias);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -280,19 +283,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::tc_commit_pair(acc_full(acc), pair_mask);
     }
   } else if (warp >= 4) {
-    // ---- Epilogue: warp w holds tile rows 32 (w % 4) .. + 31, lane = row.
+    // ---- Epilogue: warp 4 + 4 h + w holds tile rows 32 w .. + 31, lane = row,
+    // and every other unit of 32 columns.
     const int w = warp & 3;
+    const int half = (warp >> 2) - 1;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(w * 32) << 16);
-    uint8_t* slots = staging + w * kSlots * kSlotBytes;
-    float* sbias = bias_smem + w * 64;
+    uint8_t* slots = staging + (warp - 4) * kSlots * kSlotBytes;
+    T* sbias = bias_smem + (warp - 4) * 64;
     const bool keep = args.pre[0] != nullptr;
+    const bool biased = args.bias[0] != nullptr || args.bias[1] != nullptr;
     const T* res = static_cast<const T*>(args.residual);
-    // Staging buffers a column chunk fills: the output and what is kept.
-    const int per_chunk = 1 + (keep ? (GATED ? 2 : 1) : 0);
+    // Staging buffers a unit fills: the output and what is kept.
+    const int per_unit = 1 + (keep ? (GATED ? 2 : 1) : 0);
+    // This warp's units of a tile; a split tile's are shared by its pairs.
+    const int first_col = SPLIT ? 32 * (2 * range + half) : 32 * half;
+    const int col_step = SPLIT ? 64 * split : 64;
     int slot = 0, local = 0;
     bool joined = false;
     for (int t = first_tile; t < num_tiles; t += tile_step, ++local) {
       const int acc = local & 1;
+      const Tile tile = tile_at<kTileN>(args, t);
+      const int row0 = tile.m0 + static_cast<int>(rank) * 128 + w * 32;
+      const int row = row0 + lane;
+      // The residual of a unit is requested one unit ahead, the tile's first
+      // before its accumulator is waited for.
+      uint4 ahead[4] = {};
+      [[maybe_unused]] auto request = [&](int c) {
+        const int u0 = tile.n0 + c;
+        if (!GATED && res != nullptr && args.residual_vec && c < kTileN && row < args.m && u0 + 32 <= args.n) {
+          const uint4* rp = reinterpret_cast<const uint4*>(res + static_cast<long long>(row) * args.ld_residual + u0);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) ahead[q] = rp[q];
+        }
+      };
+      request(first_col);
       const bool ready =
           ptx::mbar_wait_bounded(acc_full(acc), (local >> 1) & 1, abort_flag, kWaitBudgetNs);
       if (!__all_sync(0xffffffffu, ready)) {  // the warp leaves together
@@ -300,15 +324,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       ptx::tc_fence_after_sync();
-      const Tile tile = tile_at<kTileN>(args, t);
-      const int row0 = tile.m0 + static_cast<int>(rank) * 128 + w * 32;
-      const int row = row0 + lane;
       const uint32_t src = lane_base + acc * BN;
       if constexpr (SPLIT) {
         // FP32 partials into the drained ring: [group of 4 columns][tile row].
         float4* part = reinterpret_cast<float4*>(smem) + w * 32 + lane;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
+        for (int c = 32 * half; c < BN; c += 64) {
           uint32_t r[32];
           ptx::tmem_ld_32x32b_x32(src + c, r);
           ptx::tmem_ld_wait();
@@ -353,132 +374,128 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
 #pragma unroll 1
-      for (int c = SPLIT ? 64 * range : 0; c < kTileN; c += SPLIT ? 64 * split : 64) {
-        const int col0 = tile.n0 + c;
+      for (int c = first_col; c < kTileN; c += col_step) {
+        const int u0 = tile.n0 + c;  // first output column of the unit
+        uint32_t r[32];
+        load32(c, r);
+        [[maybe_unused]] uint32_t r2[32];
+        if constexpr (GATED) load32(BN / 2 + c, r2);
         // The buffers about to be filled must have been read by their stores.
         if (lane == 0) {
-          if (per_chunk == 1) {
+          if (per_unit == 1) {
             ptx::bulk_wait_read<kSlots - 1>();
-          } else if (per_chunk == 2) {
+          } else if (per_unit == 2) {
             ptx::bulk_wait_read<kSlots - 2>();
           } else {
             ptx::bulk_wait_read<kSlots - 3>();
           }
         }
         __syncwarp();
+        if (biased) {
+          const bool in = u0 + lane < args.n;
+          const T* b0 = static_cast<const T*>(args.bias[0]);
+          sbias[lane] = b0 != nullptr && in ? b0[u0 + lane] : E::from_f(0.0f);
+          if constexpr (GATED) {
+            const T* b1 = static_cast<const T*>(args.bias[1]);
+            sbias[32 + lane] = b1 != nullptr && in ? b1[u0 + lane] : E::from_f(0.0f);
+          }
+          __syncwarp();
+        }
         uint8_t* buf[3];
 #pragma unroll
         for (int i = 0; i < 3; ++i) buf[i] = slots + ((slot + i) % kSlots) * kSlotBytes;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const int u0 = col0 + 32 * h;  // first output column of this unit
-          uint32_t r[32];
-          load32(c + 32 * h, r);
-          [[maybe_unused]] uint32_t r2[32];
-          if constexpr (GATED) load32(BN / 2 + c + 32 * h, r2);
-          __syncwarp();
-          {
-            const bool in = u0 + lane < args.n;
-            const T* b0 = static_cast<const T*>(args.bias[0]);
-            sbias[lane] = b0 != nullptr && in ? E::to_f(b0[u0 + lane]) : 0.0f;
-            if constexpr (GATED) {
-              const T* b1 = static_cast<const T*>(args.bias[1]);
-              sbias[32 + lane] = b1 != nullptr && in ? E::to_f(b1[u0 + lane]) : 0.0f;
-            }
-          }
-          __syncwarp();
-          if constexpr (!SPLIT) ptx::tmem_ld_wait();
-          if (!SPLIT && c + 64 >= kTileN && h == 1) {
-            // The accumulator is in registers: the leader may reuse it.
+        if constexpr (!SPLIT) {
+          ptx::tmem_ld_wait();
+          if (c + 64 >= kTileN) {
+            // This warp's share of the accumulator is in registers.
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(acc_empty(acc), leader));
           }
-          float v[32];
+        }
+        auto with_bias = [&](const uint32_t(&from)[32], const T* bias, float(&to)[32]) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(sbias + j);
-            v[j] = __uint_as_float(r[j]) + b.x;
-            v[j + 1] = __uint_as_float(r[j + 1]) + b.y;
-            v[j + 2] = __uint_as_float(r[j + 2]) + b.z;
-            v[j + 3] = __uint_as_float(r[j + 3]) + b.w;
-          }
-          // 16-byte chunk q of this unit in a staging buffer (128-byte swizzle).
-          auto put = [&](uint8_t* to, const float (&x)[32]) {
+          for (int j = 0; j < 32; ++j) to[j] = __uint_as_float(from[j]);
+          if (biased) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint4 p;
-              p.x = E::from_f2(x[8 * q], x[8 * q + 1]);
-              p.y = E::from_f2(x[8 * q + 2], x[8 * q + 3]);
-              p.z = E::from_f2(x[8 * q + 4], x[8 * q + 5]);
-              p.w = E::from_f2(x[8 * q + 6], x[8 * q + 7]);
-              *reinterpret_cast<uint4*>(to + lane * 128 + (((4 * h + q) ^ (lane & 7)) << 4)) = p;
-            }
-          };
-          if (keep) put(buf[1], v);
-          if constexpr (GATED) {
-            float v2[32];
+            for (int j = 0; j < 32; j += 8) {
+              const uint4 x = *reinterpret_cast<const uint4*>(bias + j);
+              const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(sbias + 32 + j);
-              v2[j] = __uint_as_float(r2[j]) + b.x;
-              v2[j + 1] = __uint_as_float(r2[j + 1]) + b.y;
-              v2[j + 2] = __uint_as_float(r2[j + 2]) + b.z;
-              v2[j + 3] = __uint_as_float(r2[j + 3]) + b.w;
-            }
-            if (keep) put(buf[2], v2);
-            with_act(args.act, [&](auto act) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = act_f<decltype(act)::value>(v[j]) * v2[j];
-            });
-          } else {
-            with_act(args.act, [&](auto act) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = act_f<decltype(act)::value>(v[j]);
-            });
-            if (res != nullptr && row < args.m) {
-              const T* rp = res + static_cast<long long>(row) * args.ld_residual + u0;
-              if (args.residual_vec && u0 + 32 <= args.n) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const uint4 x = *reinterpret_cast<const uint4*>(rp + 8 * q);
-                  const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    const float2 f = E::to_f2(xs[e]);
-                    v[8 * q + 2 * e] += f.x;
-                    v[8 * q + 2 * e + 1] += f.y;
-                  }
-                }
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  if (u0 + j < args.n) v[j] += E::to_f(rp[j]);
-                }
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = E::to_f2(xs[e]);
+                to[j + 2 * e] += f.x;
+                to[j + 2 * e + 1] += f.y;
               }
             }
           }
-          put(buf[0], v);
+        };
+        // The unit's row of this lane into a staging buffer: 64-byte swizzle.
+        auto put = [&](uint8_t* to, const float(&x)[32]) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4 p;
+            p.x = E::from_f2(x[8 * q], x[8 * q + 1]);
+            p.y = E::from_f2(x[8 * q + 2], x[8 * q + 3]);
+            p.z = E::from_f2(x[8 * q + 4], x[8 * q + 5]);
+            p.w = E::from_f2(x[8 * q + 6], x[8 * q + 7]);
+            *reinterpret_cast<uint4*>(to + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = p;
+          }
+        };
+        float v[32];
+        with_bias(r, sbias, v);
+        if (keep) put(buf[1], v);
+        if constexpr (GATED) {
+          float v2[32];
+          with_bias(r2, sbias + 32, v2);
+          if (keep) put(buf[2], v2);
+          with_act(args.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_f<decltype(act)::value>(v[j]) * v2[j];
+          });
+        } else {
+          with_act(args.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_f<decltype(act)::value>(v[j]);
+          });
+          if (res != nullptr && row < args.m) {
+            if (args.residual_vec && u0 + 32 <= args.n) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint32_t xs[4] = {ahead[q].x, ahead[q].y, ahead[q].z, ahead[q].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = E::to_f2(xs[e]);
+                  v[8 * q + 2 * e] += f.x;
+                  v[8 * q + 2 * e + 1] += f.y;
+                }
+              }
+            } else {
+              const T* rp = res + static_cast<long long>(row) * args.ld_residual + u0;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (u0 + j < args.n) v[j] += E::to_f(rp[j]);
+              }
+            }
+          }
+          request(c + col_step);
         }
+        put(buf[0], v);
         ptx::fence_proxy_async_smem();
         __syncwarp();
         // Output first, then what is kept, each its own bulk group.
         auto leave = [&](int i, const CUtensorMap* map, void* base, long long ld, bool tma) {
           if (tma) {
             if (lane == 0) {
-              if (row0 < args.m && col0 < args.n) ptx::tma_store_2d(map, ptx::smem_addr(buf[i]), col0, row0);
+              if (row0 < args.m && u0 < args.n) ptx::tma_store_2d(map, ptx::smem_addr(buf[i]), u0, row0);
               ptx::bulk_commit();
             }
           } else {
-            T* y = static_cast<T*>(base);
-            for (int rr = 0; rr < 32 && row0 + rr < args.m; ++rr) {
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int cc = lane + 32 * e;
-                if (col0 + cc < args.n) {
-                  y[static_cast<long long>(row0 + rr) * ld + col0 + cc] = *reinterpret_cast<const T*>(
-                      buf[i] + rr * 128 + (((cc >> 3) ^ (rr & 7)) << 4) + (cc & 7) * 2);
-                }
+            T* y = static_cast<T*>(base) + u0 + lane;
+            if (u0 + lane < args.n) {
+              for (int rr = 0; rr < 32 && row0 + rr < args.m; ++rr) {
+                y[static_cast<long long>(row0 + rr) * ld] = *reinterpret_cast<const T*>(
+                    buf[i] + rr * 64 + (((lane >> 3) ^ ((rr >> 1) & 3)) << 4) + (lane & 7) * 2);
               }
             }
             __syncwarp();
@@ -490,10 +507,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           leave(1, &maps.pre[0], args.pre[0], args.ld_pre, args.pre_tma != 0);
           if constexpr (GATED) leave(2, &maps.pre[1], args.pre[1], args.ld_pre, args.pre_tma != 0);
         }
-        slot = (slot + per_chunk) % kSlots;
+        slot = (slot + per_unit) % kSlots;
       }
     }
-    if (lane == 0) ptx::bulk_wait_all();
+    // The staging buffers have been read; the grid's end completes the writes.
+    if (lane == 0) ptx::bulk_wait_read<0>();
     // An aborted epilogue still takes its part in the join's barrier.
     if (SPLIT && !joined) {
       ptx::cluster_arrive_release();
@@ -557,9 +575,9 @@ cudaError_t launch_typed(const Product& p, int split, int sm_count, unsigned int
     // A map that no store uses repeats an operand's.
     maps.out[i] = maps.a[0];
     maps.pre[i] = maps.a[0];
-    if (args.out_tma) ok = ok && encode_tile_map(&maps.out[i], p.dtype, args.out[i], p.m, p.n, p.ld_out, 32);
+    if (args.out_tma) ok = ok && encode_tile_map(&maps.out[i], p.dtype, args.out[i], p.m, p.n, p.ld_out, 32, 32);
     if (args.pre_tma && args.pre[i] != nullptr) {
-      ok = ok && encode_tile_map(&maps.pre[i], p.dtype, args.pre[i], p.m, p.n, p.ld_pre, 32);
+      ok = ok && encode_tile_map(&maps.pre[i], p.dtype, args.pre[i], p.m, p.n, p.ld_pre, 32, 32);
     }
   }
   if (!ok) return cudaErrorInvalidValue;
@@ -644,30 +662,60 @@ cudaError_t set_attrs() {
   return e;
 }
 
-// Clusters of 2 * split CTAs that run at once, one CTA per SM (148 SMs in
-// GPCs of 16 to 20).
-int resident_clusters(int split, int sm_count) {
-  return split == 1 ? sm_count / 2 : split == 2 ? sm_count * 33 / 148 : split == 3 ? sm_count * 20 / 148 : sm_count * 16 / 148;
+// Clusters of 2 * split CTAs that run at once on each device (one CTA per SM;
+// a cluster stays inside a GPC), asked once per device.
+constexpr int kMaxDevices = 64;
+int g_resident[kMaxDevices][kMaxPairs + 1];
+
+cudaError_t ask_resident(int device, int sm_count) {
+  g_resident[device][1] = sm_count / 2;
+  for (int split = 2; split <= kMaxPairs; ++split) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = PairConfig<256>::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(2 * split);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(
+        &g_resident[device][split], pair_kernel<__half, false, false, 256, false, true>, &cfg);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
-// The cut with the least estimated time: waves of tiles times (K blocks per
-// range at the tile's rate, plus what a tile costs outside its main loop).
-Cut choose_cut(const Product& p, int sm_count) {
+// The cut with the least estimated time.  A K block of 64 takes a pair 0.27 us
+// whatever the tile's width (its loads through L2 bound it: 128 columns move
+// 24 KB per CTA, 256 move 32 KB, in 0.29 and 0.27 us), so a narrow tile only
+// saves epilogue (1.2 us against 2.4; 1.8 when waves follow one another), and a
+// split costs 1.5 us for the join, 3 us when a unit has two accumulators, and
+// 1.2 us more for clusters of more than two pairs.  Measured with 131 tokens:
+// 4096 x 4096, 25.9 us whole, 17.5 us in 2 ranges, 16.1 us in 3; gated 2736 x
+// 1000, 12.2 us, 10.4 us with narrow tiles, 11.2 us in 2 ranges.
+Cut choose_cut(const Product& p) {
   const bool gated = p.parts == Parts::kGated;
   const int64_t kb = (p.k + kBK - 1) / kBK * (p.parts == Parts::kConcatK ? 2 : 1);
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) return {256, 1};
   Cut best = {256, 1};
   double best_us = 0.0;
   for (int bn = 256; bn >= 128; bn /= 2) {
     const int tile_n = gated ? bn / 2 : bn;
     const int64_t tiles =
         (p.m + kTileM - 1) / kTileM * ((p.n + tile_n - 1) / tile_n) * (p.parts == Parts::kTwo ? 2 : 1);
+    const double epilogue_us = bn == 256 ? 2.4 : 1.2;
     for (int split = 1; split <= kMaxPairs && split <= kb; ++split) {
-      const int64_t at_once = std::max(resident_clusters(split, sm_count), 1);
-      const int64_t waves = (tiles + at_once - 1) / at_once;
-      const double block_us = bn == 256 ? 0.40 : 0.23;
-      const double tail_us = (bn == 256 ? 2.0 : 1.0) + (split > 1 ? 2.0 : 0.0);
-      const double us = static_cast<double>(waves) * static_cast<double>((kb + split - 1) / split) * block_us +
-                        (split > 1 ? static_cast<double>(waves) : 1.0) * tail_us;
+      const int64_t at_once = std::max(g_resident[device][split], 0);
+      if (at_once == 0 || (split > 1 && tiles > at_once)) continue;
+      const double loop_us = 0.27 * static_cast<double>((kb + split - 1) / split);
+      const double waves = static_cast<double>((tiles + at_once - 1) / at_once);
+      const double join_us = (gated ? 3.0 : 1.5) + (split > 2 ? 1.2 : 0.0);
+      const double us = split > 1 ? loop_us + epilogue_us / split + join_us
+                                  : waves * std::max(loop_us, bn == 256 ? 2.4 : 1.8) + epilogue_us;
       if (best_us == 0.0 || us < best_us) {
         best_us = us;
         best = {bn, split};
@@ -684,12 +732,16 @@ cudaError_t pair_prepare_device() {
   if (e == cudaSuccess) e = set_attrs<__half, 128>();
   if (e == cudaSuccess) e = set_attrs<__nv_bfloat16, 256>();
   if (e == cudaSuccess) e = set_attrs<__nv_bfloat16, 128>();
-  return e;
+  int device = 0, sm_count = 0;
+  if (e == cudaSuccess) e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device);
+  if (e == cudaSuccess && device >= kMaxDevices) e = cudaErrorInvalidDevice;
+  return e != cudaSuccess ? e : ask_resident(device, sm_count);
 }
 
 cudaError_t launch_pair(const Product& p, int sm_count, unsigned int* err, cudaStream_t s) {
   if (p.m < 1 || p.n < 1 || p.k < 1) return cudaErrorInvalidValue;
-  Cut cut = choose_cut(p, sm_count);
+  Cut cut = choose_cut(p);
   return p.dtype == GLQ_DTYPE_BF16 ? launch_cut<__nv_bfloat16>(p, cut, sm_count, err, s)
                                    : launch_cut<__half>(p, cut, sm_count, err, s);
 }

@@ -13,10 +13,13 @@
 //     MMA computes both projections and the activations' product is formed
 //     inside the CTA.
 //   * Join: each CTA leaves its FP32 partial tile in its drained load ring as
-//     [group of 4 tokens][row]; after a cluster barrier the CTAs of the
-//     cluster each take a share of the groups, read the S partials through
-//     distributed shared memory and add them in split order, so the result
-//     does not depend on timing.
+//     [group of 4 tokens][row]; the CTAs of the cluster each own a share of
+//     the groups and add the S partials in split order, so the result does not
+//     depend on timing.  Up to 64 tokens the partials are pushed, one bulk
+//     copy per owner, completing on the owner's barrier (1 x 4096 x 4096: 9.3
+//     us when owners read them through distributed shared memory between two
+//     cluster barriers); the receive buffer of 128 tokens would cost the second
+//     CTA per SM, so those are read.
 //   * The epilogue (bias, activation, product, residual) runs on those sums
 //     in FP32 with one rounding per output.
 // The same kernel computes the input gradient for few tokens (W MN-major, and
@@ -44,10 +47,13 @@ struct SkinnyConfig {
   static constexpr uint32_t kWBytes = kRows * kBK * 2;
   static constexpr uint32_t kABytes = BT * kBK * 2;
   static constexpr uint32_t kStageBytes = kWBytes + kABytes;
-  static constexpr int kStages = BT == 16 ? 6 : BT == 32 ? 5 : BT == 64 ? 4 : 3;
+  static constexpr int kStages = BT == 16 ? 5 : BT == 32 ? 4 : 3;
   static constexpr uint32_t kRing = kStages * kStageBytes;
-  static constexpr int kBars = 2 * kStages + 1;
-  static constexpr uint32_t kSmem = 1024 + kRing + kBars * 8 + 16;
+  static constexpr bool kPush = BT <= 64;
+  // Largest receive buffer: split - 1 partials of ceil(BT / 4 / split) groups.
+  static constexpr uint32_t kReceive = !kPush ? 0 : BT <= 32 ? 7 * kRows * 16 : 7 * 2 * kRows * 16;
+  static constexpr int kBars = 2 * kStages + 2;
+  static constexpr uint32_t kSmem = 1024 + kRing + kReceive + kBars * 8 + 16;
   static constexpr uint32_t kTmemCols = BT < 32 ? 32 : BT;
   static_assert(kSmem <= kTwoPerSm, "two CTAs per SM");
   static_assert(kRows * BT * 4 <= kRing, "the partial tile reuses the ring");
@@ -86,12 +92,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
   uint8_t* smem = smem_dyn + pad;
   const uint32_t sbase = raw + pad;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kRing);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kRing + Cfg::kReceive);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto full_bar = [&](int i) { return ptx::smem_addr(&bars[i]); };
   auto empty_bar = [&](int i) { return ptx::smem_addr(&bars[kStages + i]); };
   const uint32_t done_bar = ptx::smem_addr(&bars[2 * kStages]);
+  const uint32_t receive_bar = ptx::smem_addr(&bars[2 * kStages + 1]);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -102,6 +109,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int kb_begin = static_cast<int>(static_cast<long long>(s) * args.kb_total / split);
   const int kb_end = static_cast<int>(static_cast<long long>(s + 1) * args.kb_total / split);
   const int nkb = kb_end - kb_begin;
+  // The groups of 4 tokens that rank q of the cluster joins: [share(q),
+  // share(q + 1)).
+  const int tokens = min(BT, args.m - m0);
+  const int groups = (tokens + 3) >> 2;
+  auto share = [&](int q) { return q * groups / split; };
+  const int own_lo = share(s);
+  const int own = share(s + 1) - own_lo;
   auto raise = [&](unsigned int bit) {
     atomicOr(args.err, bit);
     *abort_flag = 1;
@@ -144,8 +158,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       ptx::mbar_init(empty_bar(i), 1);
     }
     ptx::mbar_init(done_bar, 1);
+    ptx::mbar_init(receive_bar, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
+    if (Cfg::kPush && split > 1) {
+      ptx::mbar_arrive_expect_tx(receive_bar, static_cast<uint32_t>((split - 1) * own * kRows * 16));
+    }
     if (nkb > 0) {
       ptx::prefetch_tensormap(&maps.w[0]);
       ptx::prefetch_tensormap(&maps.a[0]);
@@ -173,6 +191,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   ptx::tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
+  // Waited for after the main loop: every receive barrier is initialised.
+  if (Cfg::kPush && split > 1) ptx::cluster_arrive_relaxed();
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
@@ -218,8 +238,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   ptx::tc_fence_after_sync();
 
   // ---- Partial tile to shared memory: [group of 4 tokens][row], 16 bytes each.
-  const int tokens = min(BT, args.m - m0);
-  const int groups = (tokens + 3) >> 2;
   {
     const int row = (warp & 3) * 32 + lane;
     const uint32_t src = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -243,19 +261,55 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
   }
-  __syncthreads();
-  if (split > 1) ptx::cluster_sync();
+  bool joined = true;
+  if (split > 1) {
+    if constexpr (Cfg::kPush) {
+      ptx::cluster_wait();
+      ptx::fence_proxy_async_smem();
+      __syncthreads();
+      // Lane d ships the groups of rank s + d, so every owner is fed by a
+      // different source at any moment; sources take receive slots in rank
+      // order.
+      if (warp == 0 && lane >= 1 && lane < split && !aborted) {
+        const int owner = (s + lane) % split;
+        const uint32_t bytes = static_cast<uint32_t>((share(owner + 1) - share(owner)) * kRows * 16);
+        if (bytes > 0) {
+          const uint32_t slot = static_cast<uint32_t>(s < owner ? s : s - 1);
+          ptx::bulk_copy_to_peer(ptx::map_to_rank(sbase + Cfg::kRing + slot * bytes, owner),
+                                 sbase + static_cast<uint32_t>(share(owner) * kRows * 16), bytes,
+                                 ptx::map_to_rank(receive_bar, owner));
+        }
+      }
+      joined = ptx::mbar_wait_bounded(receive_bar, 0, aborted ? abort_flag : nullptr, kWaitBudgetNs);
+      if (!joined && !aborted) raise(kErrTimeoutEpilogue);
+      // Arriving only after its own copies have landed, every CTA knows at
+      // the last wait that none is in flight.
+      ptx::cluster_arrive_relaxed();
+    } else {
+      __syncthreads();
+      ptx::cluster_sync();
+    }
+  } else {
+    __syncthreads();
+  }
 
   // ---- Join and epilogue: this CTA's share of the groups.
-  const int own_lo = s * groups / split;
-  const int own = (s + 1) * groups / split - own_lo;
-  auto total = [&](int group, int row) {
+  auto total = [&](int j, int row) {
+    const int group = own_lo + j;
+    const float4* mine = reinterpret_cast<const float4*>(smem) + group * kRows + row;
+    if (split == 1) return *mine;
     const uint32_t at = sbase + static_cast<uint32_t>((group * kRows + row) * 16);
-    if (split == 1) return *reinterpret_cast<const float4*>(smem + (group * kRows + row) * 16);
+    const float4* received = reinterpret_cast<const float4*>(smem + Cfg::kRing) + j * kRows + row;
     float4 part[GLQ_MAX_SPLIT];
 #pragma unroll
     for (int src = 0; src < GLQ_MAX_SPLIT; ++src) {
-      if (src < split) part[src] = ptx::ld_dsmem_v4(ptx::map_to_rank(at, src));
+      if (src < split) {
+        if constexpr (Cfg::kPush) {
+          part[src] = src == s ? *mine : received[(src < s ? src : src - 1) * own * kRows];
+        } else {
+          part[src] = ptx::ld_dsmem_v4(ptx::map_to_rank(at, src));
+        }
+      }
     }
     float4 acc = part[0];
 #pragma unroll
@@ -272,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   T* out = static_cast<T*>(args.out);
   const T* res = static_cast<const T*>(args.residual);
   const bool keep = args.pre[0] != nullptr;
-  if (!aborted) {
+  if (!aborted && joined) {
     const int row = threadIdx.x % kOutRows;
     const int n = n0 + row;
     const bool n_ok = n < args.n;
@@ -280,18 +334,17 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (n_ok && args.bias[0] != nullptr) b0 = E::to_f(static_cast<const T*>(args.bias[0])[n]);
     if (GATED && n_ok && args.bias[1] != nullptr) b1 = E::to_f(static_cast<const T*>(args.bias[1])[n]);
     for (int j = threadIdx.x / kOutRows; j < own; j += kThreads / kOutRows) {
-      const int group = own_lo + j;
-      const float4 t0 = total(group, row);
+      const float4 t0 = total(j, row);
       float v[4] = {t0.x + b0, t0.y + b0, t0.z + b0, t0.w + b0};
       [[maybe_unused]] float v2[4];
       if constexpr (GATED) {
-        const float4 t1 = total(group, kOutRows + row);
+        const float4 t1 = total(j, kOutRows + row);
         v2[0] = t1.x + b1;
         v2[1] = t1.y + b1;
         v2[2] = t1.z + b1;
         v2[3] = t1.w + b1;
       }
-      const int m = m0 + 4 * group;
+      const int m = m0 + 4 * (own_lo + j);
       if (keep && n_ok) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -333,7 +386,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
-  if (split > 1) ptx::cluster_sync();  // the peers have read this CTA's partials
+  if (split > 1) {  // the peers have this CTA's partials
+    if constexpr (Cfg::kPush) {
+      ptx::cluster_wait();
+    } else {
+      ptx::cluster_sync();
+    }
+  }
   if (warp == 1) {
     ptx::tc_fence_after_sync();
     ptx::tmem_dealloc(tmem, Cfg::kTmemCols);

@@ -58,7 +58,6 @@
 #include <algorithm>
 #include <mutex>
 
-#include "glq_ffn.h"
 #include "glq_internal.h"
 #include "glq_ptx.cuh"
 
@@ -1484,13 +1483,6 @@ cudaError_t launch_bt(const Problem& p, int split, int tile_t, int tile_n, int s
 }
 
 }  // namespace
-
-bool encode_tile_map(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t cols, int64_t pitch,
-                     uint32_t box_rows) {
-  const CUtensorMapDataType type =
-      dtype == GLQ_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return encode_2d(map, type, base, cols, rows, pitch * 2, kTileK, box_rows);
-}
 
 cudaError_t tc_prepare_device() {
   cudaError_t e = set_attrs_all<__half>();

@@ -245,7 +245,10 @@ def test_outputs_touch_nothing_else(m, n, pad, off):
     assert torch.equal(y, ffn.fused_linear(a, b, None, "gelu"))
     want = ffn.gated_linear(a, b, b2, None, None, "gelu", return_preact=True)
     assert all(torch.equal(x, w) for x, w in zip((h, g, u), want))
-    assert torch.equal(z, g) and torch.equal(nv, ffn.layer_norm(z))
+    # z and gate are the same sums, cut up for different kernels: each within its own bound.
+    _, wz, _, ez = ref.linear(d(a), d(b), None, "gelu", None, F16)
+    ref.within(z, wz, ez, "z")
+    assert torch.equal(nv, ffn.layer_norm(z))
     for buf, v in bufs + [(nbuf, nv)]:
         v.fill_(123.0)
         assert bool((buf == 123.0).all())
@@ -364,11 +367,12 @@ def test_block_runs_and_trains(m):
     doubles = [t.double().requires_grad_() for t in leaves]
     want = block(reference, *doubles)
     want.backward(dy.double())
+    want = want.detach()
     # Four 16-bit roundings lie on the path of y (norm, h, and y itself; gate and up stay in 32 bits), up to eight
     # on a gradient's; each is half a step at most of values of the result's own size, so in the 2-norm their sum
     # stays below their number times the unit.
     u = ref.unit(dtype)
-    assert float((y.double() - want).norm() / want.norm()) <= 4 * u
+    assert float((y.detach().double() - want).norm() / want.norm()) <= 4 * u
     for p, q in zip(params, doubles):
         assert p.grad.dtype == dtype and p.grad.shape == q.grad.shape
         assert float((p.grad.double() - q.grad).norm() / q.grad.norm()) <= 8 * u
