@@ -55,10 +55,25 @@ struct Product {
 // Largest token count of the skinny kernel's one-pass tiles.
 constexpr int kSkinnyTokens = 128;
 
-// One call of the pair kernel (any m) or of the skinny kernel (k-major A;
-// parts other than kTwo).  m, n >= 1; k >= 0 for the skinny kernel, k >= 1
-// for the pair kernel.
-cudaError_t launch_pair(const Product& p, int sm_count, unsigned int* err, cudaStream_t s);
+// How a launch of the pair kernel is scheduled (see glq_pair.cu).
+struct PairPlan {
+  int pairs = 0;           // CTA pairs launched
+  int split = 1;           // pairs per cluster that share a tile's K range
+  int64_t whole = 0;       // tiles of the first product computed whole
+  int runs = 0;            // pairs that the other tiles' K blocks are dealt to
+  int64_t run_blocks = 0;  // those blocks
+  size_t workspace_bytes = 0;
+  double us = 0.0;         // estimate, after the launch
+};
+PairPlan plan_pair(const Product* products, int count, int sm_count);
+bool share_launch(const Product* products, int sm_count);
+
+// One launch of the pair kernel for one product (any m, k >= 1), or for two
+// without epilogue of their own; workspace: plan_pair's bytes, 256-byte
+// aligned.
+cudaError_t launch_pair(const Product* products, int count, void* workspace, int sm_count, unsigned int* err,
+                        cudaStream_t s);
+// One call of the skinny kernel: k-major A, parts other than kTwo, k >= 0.
 cudaError_t launch_skinny(const Product& p, int sm_count, unsigned int* err, cudaStream_t s);
 cudaError_t pair_prepare_device();
 cudaError_t skinny_prepare_device();

@@ -7,6 +7,7 @@
 // its operator, with an arena that only counts.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdint>
 
@@ -111,12 +112,32 @@ int check_workspace(const Arena& need, const void* workspace, size_t bytes) {
   return workspace == nullptr || !aligned(workspace, 256) || bytes < need.used ? GLQ_ERR_WORKSPACE : GLQ_OK;
 }
 
+// The current device's SM count (148 without one: sizes can be asked anywhere).
+int device_sms() {
+  int sm_count = 0;
+  unsigned int* err = nullptr;
+  return current_device(&sm_count, &err) == GLQ_OK ? sm_count : 148;
+}
+
+// Few tokens (or no sums at all): the skinny kernel, which wants A k-major.
+bool is_skinny(const Product& p) {
+  if (p.parts == Parts::kTwo) return false;
+  return p.k == 0 || (p.m <= kSkinnyTokens && p.a[0].k_major);
+}
+
+size_t product_workspace(const Product& p, int sm_count) {
+  return is_skinny(p) ? 0 : plan_pair(&p, 1, sm_count).workspace_bytes;
+}
+
+// The pitch of a single row means nothing: one the TMA takes.
+void settle_pitches(Product* p) {
+  if (p->m == 1) p->ld_out = p->ld_pre = p->ld_residual = repack_pitch(p->n);
+}
+
 // One product by the kernel for its size.
-cudaError_t run_product(Product p, int sm_count, unsigned int* err, cudaStream_t s) {
-  // The pitch of a single row means nothing: one the TMA takes.
-  if (p.m == 1) p.ld_out = p.ld_pre = p.ld_residual = repack_pitch(p.n);
-  const bool skinny = p.parts != Parts::kTwo && (p.k == 0 || p.a[0].k_major) && (p.k == 0 || p.m <= kSkinnyTokens);
-  return skinny ? launch_skinny(p, sm_count, err, s) : launch_pair(p, sm_count, err, s);
+cudaError_t run_product(Product p, void* workspace, int sm_count, unsigned int* err, cudaStream_t s) {
+  settle_pitches(&p);
+  return is_skinny(p) ? launch_skinny(p, sm_count, err, s) : launch_pair(&p, 1, workspace, sm_count, err, s);
 }
 
 // rows x cols zeros.
@@ -129,42 +150,42 @@ cudaError_t zero_rows(void* p, int64_t rows, int64_t cols, int64_t ld, cudaStrea
 
 // ---- forward
 
-// The operands of a forward call: A k-major, the weights in one order.
+// A forward call's operands (A k-major, the weights in one order) and the
+// product's workspace.
 struct ForwardPlan {
-  Operand a, b[2];
   Copies copies;
+  void* workspace = nullptr;
 };
 
-ForwardPlan plan_forward(const Matrix& a, const Matrix& b0, const Matrix* b1, Arena* arena) {
-  ForwardPlan p;
-  p.a = operand(a, Major::kK, arena, &p.copies);
-  p.b[0] = operand(b0, Major::kAny, arena, &p.copies);
-  if (b1 != nullptr) p.b[1] = operand(*b1, p.b[0].k_major ? Major::kK : Major::kMn, arena, &p.copies);
-  return p;
+ForwardPlan plan_forward(Product* p, const Matrix& a, const Matrix& b0, const Matrix* b1, int sm_count,
+                         Arena* arena) {
+  ForwardPlan plan;
+  p->a[0] = operand(a, Major::kK, arena, &plan.copies);
+  p->b[0] = operand(b0, Major::kAny, arena, &plan.copies);
+  if (b1 != nullptr) p->b[1] = operand(*b1, p->b[0].k_major ? Major::kK : Major::kMn, arena, &plan.copies);
+  plan.workspace = arena->take(product_workspace(*p, sm_count));
+  return plan;
 }
 
 int run_forward(Product p, const Matrix& a, const Matrix& b0, const Matrix* b1, void* workspace, size_t bytes,
                 cudaStream_t s) {
-  Arena arena;
+  int sm_count = device_sms();
   ForwardPlan plan;
   if (p.k > 0) {
-    plan = plan_forward(a, b0, b1, &arena);
+    Arena arena;
+    plan_forward(&p, a, b0, b1, sm_count, &arena);
     const int w = check_workspace(arena, workspace, bytes);
     if (w != GLQ_OK) return w;
     arena = Arena{static_cast<unsigned char*>(workspace), 0};
-    plan = plan_forward(a, b0, b1, &arena);
-    p.a[0] = plan.a;
-    p.b[0] = plan.b[0];
-    p.b[1] = plan.b[1];
+    plan = plan_forward(&p, a, b0, b1, sm_count, &arena);
   }
-  int sm_count = 0;
   unsigned int* err = nullptr;
   const int d = current_device(&sm_count, &err);
   if (d != GLQ_OK) return d;
   // A copied weight is written just before the product reads it.
   if (plan.copies.count > 0) p.flags &= ~static_cast<unsigned int>(GLQ_FLAG_STATIC_WEIGHTS);
   cudaError_t e = run_copies(plan.copies, sm_count, s);
-  if (e == cudaSuccess) e = run_product(p, sm_count, err, s);
+  if (e == cudaSuccess) e = run_product(p, plan.workspace, sm_count, err, s);
   return status_of(e);
 }
 
@@ -200,13 +221,15 @@ bool gradient_nk(const Backward& q) { return q.db_ks == 1 && (q.n == 1 || q.db_n
 struct BackwardPlan {
   bool make_dz;       // dz is written to the workspace (else it is dy)
   Operand dz[2];      // rows m, contraction n
-  Operand b[2];       // rows k, contraction n
-  Operand a;          // rows k, contraction m
   float* part = nullptr;
   Copies copies;
+  Product products[2];  // the input's gradient, the weights' gradient
+  int count = 0;
+  bool together = false;  // one launch
+  void* workspace = nullptr;
 };
 
-BackwardPlan plan_backward(const Backward& q, int sm_count, Arena* arena) {
+BackwardPlan plan_backward(const Backward& q, unsigned int flags, int sm_count, Arena* arena) {
   BackwardPlan p;
   const int pair = q.gated ? 2 : 1;
   const Matrix dy = {q.dy, q.m, q.n, q.ld_dy, 1};
@@ -221,11 +244,46 @@ BackwardPlan plan_backward(const Backward& q, int sm_count, Arena* arena) {
     p.dz[0] = {q.dy, row_pitch(dy), true};
   }
   if (products && q.want_da) {
-    p.b[0] = operand(q.b[0], Major::kAny, arena, &p.copies);
-    if (q.gated) p.b[1] = operand(q.b[1], p.b[0].k_major ? Major::kK : Major::kMn, arena, &p.copies);
+    Product& r = p.products[p.count++];
+    r.parts = q.gated ? Parts::kConcatK : Parts::kOne;
+    r.m = q.m;
+    r.n = q.k;
+    r.k = q.n;
+    r.out[0] = q.da;
+    r.ld_out = q.ld_da;
+    r.b[0] = operand(q.b[0], Major::kAny, arena, &p.copies);
+    if (q.gated) r.b[1] = operand(q.b[1], r.b[0].k_major ? Major::kK : Major::kMn, arena, &p.copies);
+    for (int i = 0; i < pair; ++i) r.a[i] = p.dz[i];
   }
-  if (products && q.want_db) p.a = operand(transposed(q.a), Major::kMn, arena, &p.copies);
+  if (products && q.want_db) {
+    // dB^T [n, k] = dz^T A, or dB [k, n] = A^T dz: rows as the gradient lies.
+    const bool nk = gradient_nk(q);
+    const Operand a = operand(transposed(q.a), Major::kMn, arena, &p.copies);
+    Product& r = p.products[p.count++];
+    r.parts = q.gated ? Parts::kTwo : Parts::kOne;
+    r.m = nk ? q.n : q.k;
+    r.n = nk ? q.k : q.n;
+    r.k = q.m;
+    r.ld_out = nk ? q.db_ns : q.db_ks;
+    for (int i = 0; i < pair; ++i) {
+      const Operand dz = {p.dz[i].base, p.dz[i].pitch, false};
+      r.a[i] = nk ? dz : a;
+      r.b[i] = nk ? a : dz;
+      r.out[i] = q.db[i];
+    }
+  }
   if (q.want_dbias) p.part = static_cast<float*>(arena->take(act_backward_partial_bytes(q.m, q.n, pair, sm_count)));
+  for (int i = 0; i < p.count; ++i) {
+    p.products[i].dtype = q.dtype;
+    p.products[i].flags = flags;
+    settle_pitches(&p.products[i]);
+  }
+  p.together = p.count == 2 && !is_skinny(p.products[0]) && share_launch(p.products, sm_count);
+  // Launches follow one another, so they share it; a size that was asked for
+  // both gradients serves a call for one.
+  size_t bytes = p.together ? plan_pair(p.products, 2, sm_count).workspace_bytes : 0;
+  for (int i = 0; i < p.count; ++i) bytes = std::max(bytes, product_workspace(p.products[i], sm_count));
+  p.workspace = arena->take(bytes);
   return p;
 }
 
@@ -246,13 +304,13 @@ int run_backward(const Backward& q, unsigned int flags, void* workspace, size_t 
     }
     return status_of(e);
   }
+  flags &= ~static_cast<unsigned int>(GLQ_FLAG_STATIC_WEIGHTS);
   Arena arena;
-  plan_backward(q, sm_count, &arena);
+  plan_backward(q, flags, sm_count, &arena);
   const int w = check_workspace(arena, workspace, bytes);
   if (w != GLQ_OK) return w;
   arena = Arena{static_cast<unsigned char*>(workspace), 0};
-  const BackwardPlan p = plan_backward(q, sm_count, &arena);
-  flags &= ~static_cast<unsigned int>(GLQ_FLAG_STATIC_WEIGHTS);
+  const BackwardPlan p = plan_backward(q, flags, sm_count, &arena);
 
   cudaError_t e = cudaSuccess;
   if (p.make_dz || q.want_dbias) {
@@ -272,40 +330,12 @@ int run_backward(const Backward& q, unsigned int flags, void* workspace, size_t 
     e = launch_act_backward(q.dtype, q.gated, a, q.dbias, sm_count, flags, s);
   }
   if (e == cudaSuccess) e = run_copies(p.copies, sm_count, s);
-  if (e == cudaSuccess && q.want_da && q.k > 0) {
-    Product r;
-    r.dtype = q.dtype;
-    r.parts = q.gated ? Parts::kConcatK : Parts::kOne;
-    r.m = q.m;
-    r.n = q.k;
-    r.k = q.n;
-    r.out[0] = q.da;
-    r.ld_out = q.ld_da;
-    r.flags = flags;
-    for (int i = 0; i < pair; ++i) {
-      r.a[i] = p.dz[i];
-      r.b[i] = p.b[i];
+  if (p.together) {
+    if (e == cudaSuccess) e = launch_pair(p.products, 2, p.workspace, sm_count, err, s);
+  } else {
+    for (int i = 0; i < p.count && e == cudaSuccess; ++i) {
+      e = run_product(p.products[i], p.workspace, sm_count, err, s);
     }
-    e = run_product(r, sm_count, err, s);
-  }
-  if (e == cudaSuccess && q.want_db && q.k > 0) {
-    // dB^T [n, k] = dz^T A, or dB [k, n] = A^T dz: rows as the gradient lies.
-    const bool nk = gradient_nk(q);
-    Product r;
-    r.dtype = q.dtype;
-    r.parts = q.gated ? Parts::kTwo : Parts::kOne;
-    r.m = nk ? q.n : q.k;
-    r.n = nk ? q.k : q.n;
-    r.k = q.m;
-    r.ld_out = nk ? q.db_ns : q.db_ks;
-    r.flags = flags;
-    for (int i = 0; i < pair; ++i) {
-      const Operand dz = {p.dz[i].base, p.dz[i].pitch, false};
-      r.a[i] = nk ? dz : p.a;
-      r.b[i] = nk ? p.a : dz;
-      r.out[i] = q.db[i];
-    }
-    e = run_product(r, sm_count, err, s);
   }
   return status_of(e);
 }
@@ -333,12 +363,6 @@ int check_backward(const Backward& q) {
   if (q.k > 0 && q.want_db && q.a.ptr == nullptr) return GLQ_ERR_INVALID_ARGUMENT;
   if (bad_pitch(q.dy, q.m, q.n, q.ld_dy)) return GLQ_ERR_SHAPE;
   return GLQ_OK;
-}
-
-int device_sms() {
-  int sm_count = 0;
-  unsigned int* err = nullptr;
-  return current_device(&sm_count, &err) == GLQ_OK ? sm_count : 148;
 }
 
 }  // namespace
@@ -387,9 +411,13 @@ size_t glq_fused_linear_workspace_bytes(int dtype, const void* A, int64_t a_row_
                                         const void* B, int64_t b_k_stride, int64_t b_n_stride, int64_t M, int64_t N,
                                         int64_t K) {
   if (glq::check_common(dtype, GLQ_ACT_NONE, M, N, K, 0) != GLQ_OK || M == 0 || N == 0 || K == 0) return 0;
+  Product p;
+  p.m = M;
+  p.n = N;
+  p.k = K;
   glq::Arena arena;
-  glq::plan_forward(Matrix{A, M, K, a_row_stride, a_col_stride}, glq::weight_rows(B, b_k_stride, b_n_stride, N, K),
-                    nullptr, &arena);
+  glq::plan_forward(&p, Matrix{A, M, K, a_row_stride, a_col_stride},
+                    glq::weight_rows(B, b_k_stride, b_n_stride, N, K), nullptr, glq::device_sms(), &arena);
   return arena.used;
 }
 
@@ -433,10 +461,15 @@ size_t glq_gated_linear_workspace_bytes(int dtype, const void* A, int64_t a_row_
                                         const void* Bg, int64_t bg_k_stride, int64_t bg_n_stride, const void* Bu,
                                         int64_t bu_k_stride, int64_t bu_n_stride, int64_t M, int64_t N, int64_t K) {
   if (glq::check_common(dtype, GLQ_ACT_NONE, M, N, K, 0) != GLQ_OK || M == 0 || N == 0 || K == 0) return 0;
+  Product p;
+  p.parts = Parts::kGated;
+  p.m = M;
+  p.n = N;
+  p.k = K;
   glq::Arena arena;
   const Matrix up = glq::weight_rows(Bu, bu_k_stride, bu_n_stride, N, K);
-  glq::plan_forward(Matrix{A, M, K, a_row_stride, a_col_stride},
-                    glq::weight_rows(Bg, bg_k_stride, bg_n_stride, N, K), &up, &arena);
+  glq::plan_forward(&p, Matrix{A, M, K, a_row_stride, a_col_stride},
+                    glq::weight_rows(Bg, bg_k_stride, bg_n_stride, N, K), &up, glq::device_sms(), &arena);
   return arena.used;
 }
 
@@ -489,7 +522,7 @@ size_t glq_fused_linear_backward_workspace_bytes(int dtype, const void* dY, int6
   q.want_da = q.want_db = true;
   q.want_dbias = has_bias != 0;
   glq::Arena arena;
-  glq::plan_backward(q, glq::device_sms(), &arena);
+  glq::plan_backward(q, 0, glq::device_sms(), &arena);
   return arena.used;
 }
 
@@ -551,7 +584,7 @@ size_t glq_gated_linear_backward_workspace_bytes(int dtype, const void* A, int64
   q.want_da = q.want_db = true;
   q.want_dbias = has_bias != 0;
   glq::Arena arena;
-  glq::plan_backward(q, glq::device_sms(), &arena);
+  glq::plan_backward(q, 0, glq::device_sms(), &arena);
   return arena.used;
 }
 

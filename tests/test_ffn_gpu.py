@@ -131,9 +131,12 @@ def test_fused_linear_backward(case):
     if wl in ("nk", "kn"):
         assert db.stride() == b.stride()
     only = ffn.fused_linear_backward(dy, a, b, z if act else None, act, need_b=False)
-    assert torch.equal(only[0], da) and only[1] is None and only[2] is None
+    # (the cut of the sums, and so their last bits, depend on what is asked for together)
+    ref.within(only[0], *wa, "da alone")
+    assert only[1] is None and only[2] is None
     only = ffn.fused_linear_backward(dy, a, b, z if act else None, act, need_a=False)
-    assert torch.equal(only[1], db) and only[0] is None
+    ref.within(only[1], *wb, "db alone")
+    assert only[0] is None
 
 
 @pytest.mark.parametrize("case", variants(), ids=IDS)
@@ -383,14 +386,18 @@ def test_partial_gradients():
     a, w, bias, res = make(gen, F16, 40, 64), make(gen, F16, 72, 64, scale=0.1), make(gen, F16, 72), make(gen, F16, 40, 72)
     full = [t.clone().requires_grad_() for t in (a, w, bias, res)]
     dy = make(gen, F16, 40, 72)
-    ffn.fused_linear(full[0], full[1].t(), full[2], "gelu", full[3]).backward(dy)
-    assert torch.equal(full[3].grad, dy)
+    y, z = ffn.fused_linear(full[0], full[1].t(), full[2], "gelu", full[3], return_preact=True)
+    y.backward(dy)
+    wa, (wb,), (wbias,) = ref.linear_backward(d(dy), d(a), d(w.t()), d(z.detach()), "gelu", F16)
+    want = [wa, (wb[0].t(), wb[1].t()), wbias, (d(dy), torch.zeros_like(d(dy)))]
+    for t, v in zip(full, want):
+        ref.within(t.grad, *v, "gradient")
     for i in range(4):
         some = [t.clone().requires_grad_(j == i) for j, t in enumerate((a, w, bias, res))]
         ffn.fused_linear(some[0], some[1].t(), some[2], "gelu", some[3]).backward(dy)
         for j, t in enumerate(some):
             assert (t.grad is None) == (j != i)
-        assert torch.equal(some[i].grad, full[i].grad)
+        ref.within(some[i].grad, *want[i], "gradient alone")
 
 
 def test_custom_ops_check():
