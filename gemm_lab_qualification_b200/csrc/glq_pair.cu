@@ -34,10 +34,6 @@
 //     Neither join depends on timing.
 //   * Two products may share a launch (the input's and the weights' gradients):
 //     together they fill waves that each alone would leave ragged.
-//   * The ring is as deep as shared memory allows (6 stages of 32 KB per CTA):
-//     a stage's round trip through L2 takes about 1.4 us, so its depth, not the
-//     tensor pipe, sets the pace of an unthrottled chip (5 stages: 0.27 us per
-//     K block).
 //   * Operands are K-major or MN-major (the transposed operands of the
 //     backward products), both read by TMA as they lie in memory: no
 //     transposition pass.
@@ -68,14 +64,14 @@ constexpr int kBK = 64;         // K elements per stage: one 128-byte swizzle ro
 constexpr int kThreads = 384;
 constexpr int kTileM = 256;     // rows per pair
 constexpr int kEpiWarps = 8;    // warps 4..11, two per 32 TMEM lanes
-constexpr int kSlots = 2;       // staging buffers per epilogue warp
+constexpr int kSlots = 4;       // staging buffers per epilogue warp: a tile's units, or a unit's outputs
 constexpr int kMaxPairs = 4;    // K ranges of a split tile: clusters of up to 8 CTAs
 constexpr uint32_t kSlotBytes = 32 * 64;  // a unit: 32 rows x 32 16-bit columns
 constexpr uint32_t kMnBox = 64 * kBK * 2;  // MN-major box: 64 elements x 64 K rows
 constexpr uint32_t kSmemMax = 232448;
 
 constexpr int kTileN = 256;     // accumulator columns per pair
-constexpr int kStages = 6;
+constexpr int kStages = 5;  // (6 with half the staging: no faster)
 constexpr uint32_t kOperandBytes = 128 * kBK * 2;  // a CTA's half of either operand
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
 constexpr uint32_t kRing = kStages * kStageBytes;
@@ -432,7 +428,6 @@ __global__ void __launch_bounds__(kThreads, 1)
              w * 32 + lane;
     };
     auto flag_of = [&](int r) { return args.flags + (static_cast<long long>(r) * 2 + rank) * kEpiWarps + (warp - 4); };
-    int slot = 0;
     for (int local = 0; next_piece(); ++local) {
       const PairProduct& p = args.p[piece.product];
       const int acc = local & 1;
@@ -574,6 +569,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       const bool helped = !SPLIT && piece.helpers > 0;
       if (helped) request_partial(1, first_col);
+      // Stores the unit in staging buffer `at` to its place.
+      auto leave = [&](int at, int u0, const CUtensorMap* map, void* base, long long ld, bool tma) {
+        const uint8_t* buf = slots + at * kSlotBytes;
+        if (tma) {
+          if (lane == 0 && row0 < p.m && u0 < p.n) ptx::tma_store_2d(map, ptx::smem_addr(buf), u0, row0);
+        } else if (u0 + lane < p.n) {
+          T* y = static_cast<T*>(base) + u0 + lane;
+          for (int rr = 0; rr < 32 && row0 + rr < p.m; ++rr) {
+            y[static_cast<long long>(row0 + rr) * ld] = *reinterpret_cast<const T*>(
+                buf + rr * 64 + (((lane >> 3) ^ ((rr >> 1) & 3)) << 4) + (lane & 7) * 2);
+          }
+        }
+      };
+      const CUtensorMap* out_map = &maps.out[piece.product][piece.part];
+      void* const out_base = p.out[piece.part];
+      const long long ld_out = p.ld_out;
+      const bool out_tma = p.out_tma != 0;
+      // The staging buffers have been read by the stores before.
+      auto reclaim = [&]() {
+        if (lane == 0) ptx::bulk_wait_read<0>();
+        __syncwarp();
+      };
+      reclaim();
+      int filled = 0;
 #pragma unroll 1
       for (int c = first_col; c < kOutN; c += col_step) {
         const int u0 = piece.n0 + c;  // first output column of the unit
@@ -621,13 +640,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         };
-        // The unit, row by row of lanes, into the next staging buffer (64-byte
-        // swizzle) and from there to its place, each its own bulk group.
-        auto emit = [&](const float(&x)[32], const CUtensorMap* map, void* base, long long ld, bool tma) {
-          uint8_t* buf = slots + slot * kSlotBytes;
-          slot = (slot + 1) % kSlots;
-          if (lane == 0) ptx::bulk_wait_read<kSlots - 1>();  // its last store has read it
-          __syncwarp();
+        // The unit into a staging buffer, lane = row: 64-byte swizzle.
+        auto put = [&](int at, const float(&x)[32]) {
+          uint8_t* buf = slots + at * kSlotBytes;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint4 packed;
@@ -637,32 +652,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             packed.w = E::from_f2(x[8 * q + 6], x[8 * q + 7]);
             *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = packed;
           }
-          ptx::fence_proxy_async_smem();
-          __syncwarp();
-          if (tma) {
-            if (lane == 0) {
-              if (row0 < p.m && u0 < p.n) ptx::tma_store_2d(map, ptx::smem_addr(buf), u0, row0);
-              ptx::bulk_commit();
-            }
-          } else {
-            T* y = static_cast<T*>(base) + u0 + lane;
-            if (u0 + lane < p.n) {
-              for (int rr = 0; rr < 32 && row0 + rr < p.m; ++rr) {
-                y[static_cast<long long>(row0 + rr) * ld] = *reinterpret_cast<const T*>(
-                    buf + rr * 64 + (((lane >> 3) ^ ((rr >> 1) & 3)) << 4) + (lane & 7) * 2);
-              }
-            }
-            __syncwarp();
-            if (lane == 0) ptx::bulk_commit();  // keeps the group count uniform
-          }
         };
         float v[32];
         with_bias(r, sbias, v);
-        if (keep) emit(v, &maps.pre[0], args.pre[0], args.ld_pre, args.pre_tma != 0);
+        if (keep) put(1, v);
         if constexpr (GATED) {
           float v2[32];
           with_bias(r2, sbias + 32, v2);
-          if (keep) emit(v2, &maps.pre[1], args.pre[1], args.ld_pre, args.pre_tma != 0);
+          if (keep) put(2, v2);
           with_act(args.act, [&](auto act) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = act_f<decltype(act)::value>(v[j]) * v2[j];
@@ -694,7 +691,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           request(c + col_step);
         }
-        emit(v, &maps.out[piece.product][piece.part], p.out[piece.part], p.ld_out, p.out_tma != 0);
+        put(filled, v);
+        if (keep) {
+          // A unit's outputs leave together: one fence for the three.
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          leave(0, u0, out_map, out_base, ld_out, out_tma);
+          leave(1, u0, &maps.pre[0], args.pre[0], args.ld_pre, args.pre_tma != 0);
+          if constexpr (GATED) leave(2, u0, &maps.pre[1], args.pre[1], args.ld_pre, args.pre_tma != 0);
+          if (lane == 0) ptx::bulk_commit();
+          __syncwarp();
+          reclaim();
+        } else {
+          ++filled;
+        }
+      }
+      if (!keep) {
+        // The tile's units leave together (a fence per unit made the epilogue
+        // of a 128 x 256 half tile take 4.2 us).
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        for (int i = 0; i < filled; ++i) {
+          leave(i, piece.n0 + first_col + i * col_step, out_map, out_base, ld_out, out_tma);
+        }
+        if (lane == 0) ptx::bulk_commit();
+        __syncwarp();
       }
       // The flags are left as they were found, for a replay of this launch.
       __syncwarp();
@@ -869,10 +890,10 @@ int64_t resident_clusters(int split, int sm_count) {
 }
 
 // Estimated times in us, after the launch: a K block of a tile takes 0.25, a
-// tile's epilogue 2.4; joining a split tile 1.5 (3 with two accumulators per
+// tile's epilogue 3.4; joining a split tile 1.5 (3 with two accumulators per
 // unit), 1.2 more for clusters of over two pairs; dealt runs 4.5 for the
 // hand-over and 4 for every further partial that a tile's owner adds.
-constexpr double kBlockUs = 0.25, kEpilogueUs = 2.4, kLaunchUs = 4.0;
+constexpr double kBlockUs = 0.25, kEpilogueUs = 3.4, kLaunchUs = 4.0;
 
 }  // namespace
 
@@ -910,11 +931,15 @@ PairPlan plan_pair(const Product* products, int count, int sm_count) {
   for (int64_t runs = count > 1 ? 1 : rest + 1; runs <= std::min(most, blocks); ++runs) {
     const int64_t run = (blocks + runs - 1) / runs, helpers = (longest + run - 1) / run;
     if (helpers > 16) break;  // (a warp's lanes poll one helper's flag each)
-    // A run of several short tiles runs their epilogues behind their loops.
-    const double us = whole_us +
-                      std::max(kBlockUs * static_cast<double>(run),
-                               kEpilogueUs * static_cast<double>(rest + s1.tiles) / static_cast<double>(runs)) +
-                      kEpilogueUs + 4.5 + 4.0 * static_cast<double>(helpers - 1);
+    // A run through short tiles is paced by their epilogues.
+    double loop_us = 0.0;
+    for (const Size& z : {s0, s1}) {
+      const double tiles = static_cast<double>(run) / static_cast<double>(z.kb);
+      loop_us = std::max(loop_us, tiles * std::max(kBlockUs * static_cast<double>(z.kb), tiles > 1.0 ? kEpilogueUs : 0.0));
+      if (count == 1) break;
+    }
+    const double us =
+        whole_us + loop_us + kEpilogueUs + 4.5 + 4.0 * static_cast<double>(helpers - 1);
     if (us < plan.us) {
       plan.us = us;
       best = runs;
