@@ -31,7 +31,7 @@ BENCH_BINARY = PACKAGE_DIR / "gemm_bench"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", f"-I{INCLUDE}"]
 LIBRARY_SOURCES = ["glq_api.cu", "glq_tc.cu", "glq_gemv.cu", "glq_generic.cu", "glq_ffn_api.cu", "glq_pair.cu",
-                   "glq_skinny.cu", "glq_rows.cu", "glq_tma.cu"]
+                   "glq_skinny.cu", "glq_token.cu", "glq_rows.cu", "glq_tma.cu"]
 
 
 def nvcc() -> str:

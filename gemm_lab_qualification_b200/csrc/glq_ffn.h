@@ -1,5 +1,5 @@
 // glq_ffn.h -- declarations shared by the feed-forward operators' kernels
-// (glq_pair.cu, glq_skinny.cu, glq_rows.cu) and their C-ABI layer
+// (glq_pair.cu, glq_skinny.cu, glq_token.cu, glq_rows.cu) and their C-ABI layer
 // (glq_ffn_api.cu).
 #pragma once
 
@@ -75,6 +75,9 @@ cudaError_t launch_pair(const Product* products, int count, void* workspace, int
                         cudaStream_t s);
 // One call of the skinny kernel: k-major A, parts other than kTwo, k >= 0.
 cudaError_t launch_skinny(const Product& p, int sm_count, unsigned int* err, cudaStream_t s);
+// One call of the single-token kernel: m == 1, k >= 1, every operand k-major,
+// parts kOne or kGated.
+cudaError_t launch_token(const Product& p, int sm_count, cudaStream_t s);
 cudaError_t pair_prepare_device();
 cudaError_t skinny_prepare_device();
 

@@ -125,6 +125,12 @@ bool is_skinny(const Product& p) {
   return p.k == 0 || (p.m <= kSkinnyTokens && p.a[0].k_major);
 }
 
+// One token, weights with K-contiguous rows: the single-token kernel.
+bool is_token(const Product& p) {
+  return p.m == 1 && p.k > 0 && (p.parts == Parts::kOne || p.parts == Parts::kGated) && p.a[0].k_major &&
+         p.b[0].k_major && (p.parts == Parts::kOne || p.b[1].k_major);
+}
+
 size_t product_workspace(const Product& p, int sm_count) {
   return is_skinny(p) ? 0 : plan_pair(&p, 1, sm_count).workspace_bytes;
 }
@@ -137,6 +143,7 @@ void settle_pitches(Product* p) {
 // One product by the kernel for its size.
 cudaError_t run_product(Product p, void* workspace, int sm_count, unsigned int* err, cudaStream_t s) {
   settle_pitches(&p);
+  if (is_token(p)) return launch_token(p, sm_count, s);
   return is_skinny(p) ? launch_skinny(p, sm_count, err, s) : launch_pair(&p, 1, workspace, sm_count, err, s);
 }
 

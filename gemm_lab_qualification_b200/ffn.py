@@ -56,7 +56,11 @@ def _check(status: int, what: str) -> None:
 
 
 def _differentiable(*tensors: Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ---------------------------------------------------------------- linear + bias + activation + residual
