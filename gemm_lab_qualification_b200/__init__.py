@@ -3,6 +3,8 @@
 * ``kernels`` -- the lab's operator API (``triton_matmul``,
   ``triton_bias_silu``, ``triton_splitk_matmul``, the Plans, the
   ``gemm_lab::*`` custom ops) backed by the native kernels.
+* ``ffn`` -- the feed-forward operators: linear with bias, activation and
+  residual, the gated linear pair, layer norm, each with its backward pass.
 * ``_native`` -- ctypes binding of ``libglq.so`` (C ABI in include/glq.h).
 * ``workloads`` -- the qualification contract's deterministic inputs.
 * ``evidence`` -- CUDA-event timing and statistics of the lab's harness.

@@ -39,6 +39,17 @@ int device_state(DeviceState** out) {
     return GLQ_ERR_DEVICE;
   }
   if (dev < 0 || dev >= kMaxDevices) return GLQ_ERR_DEVICE;
+  // A thread's first runtime call binds the device's context to it; encoding a
+  // tensor map, which needs the context, may come before any launch (as in the
+  // threads that run an autograd graph).
+  static thread_local int bound = -1;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) {
+      cudaGetLastError();
+      return GLQ_ERR_DEVICE;
+    }
+    bound = dev;
+  }
   DeviceState& st = g_devices[dev];
   std::call_once(st.once, [&st, dev] {
     int major = 0, minor = 0, sms = 0;

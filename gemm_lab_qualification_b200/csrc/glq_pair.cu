@@ -265,6 +265,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     atomicOr(args.err, bit);
     *abort_flag = 1;
   };
+  // Verdicts of a warp, so that its lanes stay together when a wait expires.
+  auto all_ok = [&](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+  auto going = [&]() { return all_ok(*abort_flag == 0); };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -310,11 +313,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       return walk.next(piece);
     }
   };
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // ---- TMA producer: this CTA's halves, counted on the leader's barriers.
+    // (The whole warp walks and waits, one lane issues: a loop of one lane in a
+    // diverged warp is slower.)
     int stage = 0, rounds = 0;
     const uint32_t signals = ptx::map_to_rank(full_bar(0), leader);
-    while (*abort_flag == 0 && next_piece()) {
+    while (going() && next_piece()) {
       // (in registers: the asm's memory clobbers would reload them per block)
       const PairProduct& p = args.p[piece.product];
       const int kb_part = p.kb_part;
@@ -325,7 +330,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int kb_end = piece.kb_end;
       with_orders(p, [&](auto a_mn, auto b_mn) {
         for (int kb = piece.kb_begin; kb < kb_end; ++kb) {
-          if (rounds > 0 && !ptx::mbar_wait_bounded(empty_bar(stage), (rounds - 1) & 1, abort_flag, kWaitBudgetNs)) {
+          if (!all_ok(rounds == 0 ||
+                      ptx::mbar_wait_bounded(empty_bar(stage), (rounds - 1) & 1, abort_flag, kWaitBudgetNs))) {
             raise(kErrTimeoutProducer);
             break;
           }
@@ -335,19 +341,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           const CUtensorMap* map_b = GATED ? maps_b : maps_b + half;
           const uint32_t a_dst = sbase + stage * kStageBytes;
           const uint32_t b_dst = a_dst + kOperandBytes;
-          if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * kStageBytes);
-          const uint32_t signal = signals + 8u * static_cast<uint32_t>(stage);
-          if constexpr (decltype(a_mn)::value) {
-            ptx::tma_load_2d_pair(a_dst, map_a, a_row, k0, signal);
-            ptx::tma_load_2d_pair(a_dst + kMnBox, map_a, a_row + 64, k0, signal);
-          } else {
-            ptx::tma_load_2d_pair(a_dst, map_a, k0, a_row, signal);
-          }
-          if constexpr (decltype(b_mn)::value) {
-            ptx::tma_load_2d_pair(b_dst, map_b, b_row, k0, signal);
-            ptx::tma_load_2d_pair(b_dst + kMnBox, map_b, b_row + 64, k0, signal);
-          } else {
-            ptx::tma_load_2d_pair(b_dst, map_b, k0, b_row, signal);
+          if (ptx::elect_one()) {
+            if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * kStageBytes);
+            const uint32_t signal = signals + 8u * static_cast<uint32_t>(stage);
+            if constexpr (decltype(a_mn)::value) {
+              ptx::tma_load_2d_pair(a_dst, map_a, a_row, k0, signal);
+              ptx::tma_load_2d_pair(a_dst + kMnBox, map_a, a_row + 64, k0, signal);
+            } else {
+              ptx::tma_load_2d_pair(a_dst, map_a, k0, a_row, signal);
+            }
+            if constexpr (decltype(b_mn)::value) {
+              ptx::tma_load_2d_pair(b_dst, map_b, b_row, k0, signal);
+              ptx::tma_load_2d_pair(b_dst + kMnBox, map_b, b_row + 64, k0, signal);
+            } else {
+              ptx::tma_load_2d_pair(b_dst, map_b, k0, b_row, signal);
+            }
           }
           if (++stage == kStages) {
             stage = 0;
@@ -356,20 +364,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       });
     }
-    if (*abort_flag != 0) {
+    if (lane == 0 && *abort_flag != 0) {
       // Give the copies in flight time to land before shared memory goes.
       const uint64_t t0 = ptx::globaltimer_ns();
       for (uint32_t i = 0; i < (1u << 20) && ptx::globaltimer_ns() - t0 < 2000000ull; ++i) {
       }
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     // ---- MMA issuer (leader CTA).
     int stage = 0, rounds = 0, local = 0;
     const uint16_t pair_mask = static_cast<uint16_t>(3u << leader);
-    for (; *abort_flag == 0 && next_piece(); ++local) {
+    for (; going() && next_piece(); ++local) {
       const int acc = local & 1;
-      if (local >= 2 &&
-          !ptx::mbar_wait_bounded_cluster(acc_empty(acc), ((local >> 1) - 1) & 1, abort_flag, kWaitBudgetNs)) {
+      if (!all_ok(local < 2 || ptx::mbar_wait_bounded_cluster(acc_empty(acc), ((local >> 1) - 1) & 1, abort_flag,
+                                                              kWaitBudgetNs))) {
         raise(kErrTimeoutMma);
         break;
       }
@@ -384,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // swizzled K-major row, or 16 K rows of 128 bytes.
         constexpr uint32_t kAStep = kAMn ? 128 : 2, kBStep = kBMn ? 128 : 2;
         for (int i = 0; i < blocks; ++i) {
-          if (!ptx::mbar_wait_bounded(full_bar(stage), rounds & 1, abort_flag, kWaitBudgetNs)) {
+          if (!all_ok(ptx::mbar_wait_bounded(full_bar(stage), rounds & 1, abort_flag, kWaitBudgetNs))) {
             raise(kErrTimeoutMma);
             ok = false;
             break;
@@ -393,11 +401,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t a_src = sbase + stage * kStageBytes, b_src = a_src + kOperandBytes;
           const uint64_t da = kAMn ? ptx::umma_desc_mn_sw128(a_src) : ptx::umma_desc_k_sw128(a_src);
           const uint64_t db = kBMn ? ptx::umma_desc_mn_sw128(b_src) : ptx::umma_desc_k_sw128(b_src);
+          if (ptx::elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk) {
-            ptx::tc_mma_f16_pair(d, da + kAStep * kk, db + kBStep * kk, idesc, i > 0 || kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < kBK / 16; ++kk) {
+              ptx::tc_mma_f16_pair(d, da + kAStep * kk, db + kBStep * kk, idesc, i > 0 || kk > 0 ? 1u : 0u);
+            }
+            ptx::tc_commit_pair(empty_bar(stage), pair_mask);
           }
-          ptx::tc_commit_pair(empty_bar(stage), pair_mask);
           if (++stage == kStages) {
             stage = 0;
             ++rounds;
@@ -405,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       });
       if (!ok) break;
-      ptx::tc_commit_pair(acc_full(acc), pair_mask);
+      if (ptx::elect_one()) ptx::tc_commit_pair(acc_full(acc), pair_mask);
     }
   } else if (warp >= 4) {
     // ---- Epilogue: warp 4 + 4 h + w holds tile rows 32 w .. + 31, lane = row,
@@ -445,8 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       if (!piece.partial) request(first_col);
-      bool ready = ptx::mbar_wait_bounded(acc_full(acc), (local >> 1) & 1, abort_flag, kWaitBudgetNs);
-      if (!__all_sync(0xffffffffu, ready)) {  // the warp leaves together
+      if (!all_ok(ptx::mbar_wait_bounded(acc_full(acc), (local >> 1) & 1, abort_flag, kWaitBudgetNs))) {
         if (lane == 0) raise(kErrTimeoutEpilogue);
         break;
       }
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         continue;
       }
       if (piece.helpers > 0) {
-        ready = true;
+        bool ready = true;
         if (lane < piece.helpers) {
           const unsigned long long* flag = flag_of(walk.run + 1 + lane);
           const uint64_t t0 = ptx::globaltimer_ns();
@@ -492,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (!__all_sync(0xffffffffu, ready)) {
+        if (!all_ok(ready)) {
           if (lane == 0) raise(kErrTimeoutEpilogue);
           break;
         }

@@ -23,6 +23,13 @@ the inputs' 16-bit type; every sum is FP32 with one rounding, except that the
 gradient of the pre-activations is rounded to 16 bits before the products that
 read it.  The backward passes themselves are not differentiable.
 
+Results are the same bits on every run of the same call; which gradients are
+asked for together may change the order of their sums.  All calls can be
+captured into CUDA graphs after a first call on the device.  To capture a
+``.backward()``, let no eager graph of the same leaves live at that time (torch
+keeps the leaves' gradient nodes on the stream they were made on), or capture
+the ``*_backward`` functions.
+
 The reference has no counterpart (its fused epilogue is bias + SiLU,
 kernels.py:191-249, inference only).
 """
@@ -76,7 +83,8 @@ def fused_linear_into(a: Tensor, b: Tensor, output: Tensor, bias: Tensor | None 
                       activation: str | None = None, residual: Tensor | None = None,
                       preact: Tensor | None = None) -> Tensor:
     """output = act(a @ b + bias) + residual; preact, if given, receives
-    ``a @ b + bias``.  ``output`` and ``preact`` overlap no other operand.
+    ``a @ b + bias``.  ``output`` may be the residual itself (the residual
+    stream updated in place); apart from that, outputs overlap no operand.
     Not differentiable."""
     return _fused_linear(a, b, bias, activation, residual, output, preact)[0]
 

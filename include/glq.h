@@ -360,7 +360,11 @@ enum glq_activation {
  *     0).  It holds nothing between calls: calls that may overlap need
  *     workspaces of their own.
  *   - Optional pointers may be NULL; an output that is NULL is not computed.
- *   - Outputs must not overlap inputs or each other.  flags: enum glq_flags.
+ *   - Outputs must not overlap inputs or each other, except that Y of
+ *     glq_fused_linear may be its residual (same address and row stride).
+ *   - Every sum has a fixed order, so a call gives the same bits every time;
+ *     the order depends on the sizes and on which outputs are asked for.
+ *   - flags: enum glq_flags.
  */
 
 /*

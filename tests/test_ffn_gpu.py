@@ -470,6 +470,88 @@ def test_captured_graphs(m, pdl):
                 assert all(torch.equal(p, q) for p, q in zip(out, step(x, dy)))
 
 
+def test_dealt_runs_replay():
+    """A backward pass whose K blocks are dealt over the pairs: joins through the workspace, replayed and on two
+    streams at once."""
+    gen = torch.Generator().manual_seed(12)
+    m, n, k = 999, 1032, 520
+    lib = native.library()
+    a, b = make(gen, BF16, m, k), weight(gen, BF16, k, n, "nk")
+    dy = make(gen, BF16, m, n)
+    # Aligned operands and no activation: what the workspace is for is the runs.
+    assert lib.glq_fused_linear_backward_workspace_bytes(
+        1, dy.data_ptr(), n, a.data_ptr(), k, 1, b.data_ptr(), 1, k, 0, 0, m, n, k) > 0
+    want = ffn.fused_linear_backward(dy, a, b)
+    wa, (wb,), _ = ref.linear_backward(d(dy), d(a), d(b), None, None, BF16)
+    ref.within(want[0], *wa, "da")
+    ref.within(want[1], *wb, "db")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ffn.fused_linear_backward(dy, a, b)
+        again = ffn.fused_linear_backward(dy, a, b)
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        for t in (*got[:2], *again[:2]):
+            t.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            other = ffn.fused_linear_backward(dy, a, b)
+        torch.cuda.synchronize()
+        for out in (got, again, other):
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_large_products():
+    """Whole waves and a dealt remainder; two outputs, concatenated contraction; against matmul in 64 bits."""
+    gen = torch.Generator().manual_seed(13)
+    m, n, k = 2100, 2600, 1032
+    a, bg, bu = make(gen, F16, m, k), weight(gen, F16, k, n, "nk"), weight(gen, F16, k, n, "nk")
+    dy = make(gen, F16, m, n)
+    h, g, u = ffn.gated_linear(a, bg, bu, return_preact=True)
+    wh, wg, wu, eh, eg, eu = ref.gated(d(a), d(bg), d(bu), None, None, "silu", F16)
+    for got, want, bound in ((h, wh, eh), (g, wg, eg), (u, wu, eu)):
+        ref.within(got, want, bound, "gated")
+    grads = ffn.gated_linear_backward(dy, a, bg, bu, g, u, has_bias=True)
+    wa, wb, wbias = ref.gated_backward(d(dy), d(a), d(bg), d(bu), d(g), d(u), "silu", F16)
+    for got, want in zip(grads, [wa, *wb, *wbias]):
+        ref.within(got, *want, "gradient")
+
+
+def test_a_fresh_thread():
+    """The first CUDA work of a thread may be one of these calls (an autograd thread's, for one)."""
+    import threading
+
+    gen = torch.Generator().manual_seed(15)
+    a, b, dy = make(gen, F16, 24, 64), weight(gen, F16, 64, 72, "nk"), make(gen, F16, 24, 72)
+    calls = [lambda: ffn.fused_linear_backward(dy, a, b)[:2], lambda: (ffn.gated_linear(a, b, b),),
+             lambda: (ffn.layer_norm(a),), lambda: (kernels.triton_matmul(a, b),)]
+    for call in calls:
+        want, got, errors = call(), [], []
+
+        def work():
+            try:
+                got.extend(call())
+                torch.cuda.synchronize()
+            except Exception as e:  # noqa: BLE001 -- reported below
+                errors.append(e)
+
+        thread = threading.Thread(target=work)
+        thread.start()
+        thread.join()
+        assert not errors, errors
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("m,layout", [(1, "nk"), (5, "kn"), (128, "nk"), (300, "nk")])
+def test_output_may_be_the_residual(m, layout):
+    gen = torch.Generator().manual_seed(14)
+    a, b, r = make(gen, F16, m, 264), weight(gen, F16, 264, 520, layout), make(gen, F16, m, 520)
+    want = ffn.fused_linear(a, b, activation="relu", residual=r)
+    assert ffn.fused_linear_into(a, b, r, activation="relu", residual=r) is r
+    assert torch.equal(r, want)
+
+
 def test_static_weights_flag():
     gen = torch.Generator().manual_seed(11)
     a, b, b2 = make(gen, F16, 5, 520), weight(gen, F16, 520, 264, "nk"), weight(gen, F16, 520, 264, "nk")
