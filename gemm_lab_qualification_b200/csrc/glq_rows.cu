@@ -646,19 +646,21 @@ __global__ void __launch_bounds__(32 * kSumRanges) column_sum_kernel(const Colum
 //
 // Linear: dz = dy act'(z).  Gated: dg = dy u act'(g), du = dy act(g).  One
 // block: 512 columns (8 per thread) x a strip of rows, four rows at a time;
-// each thread requests two of its rows before it works on the first, since
-// stores to dz keep the compiler from moving later loads up (4096 x 11008
-// gated: 141 us row by row).  The bias gradients' sums of the strip (of the
-// values before their rounding) stay in registers and are added over the four
-// row threads in order at the end.  The rounding of dz to 16 bits is what the
-// tensor-core products that follow read.
+// each thread has its next two rows requested while it works on one (4096 x
+// 11008 gated: 141 us row by row, since stores to dz keep the compiler from
+// moving loads up; 97 us in pairs of rows that were waited for).  SUMS: the
+// bias gradients' sums of the strip (of the values before their rounding) stay
+// in registers and are added over the four row threads in order at the end.
+// The rounding of dz to 16 bits is what the tensor-core products that follow
+// read.
 constexpr int kActCols = 64;  // column threads
 constexpr int kActRows = 4;   // row threads
 
-template <typename T, bool GATED>
-__global__ void __launch_bounds__(kActCols * kActRows) act_backward_kernel(const ActBackwardArgs a) {
+template <typename T, bool GATED, bool SUMS>
+__global__ void __launch_bounds__(kActCols * kActRows, GATED && SUMS ? 2 : 3)
+    act_backward_kernel(const ActBackwardArgs a) {
   constexpr int kSums = GATED ? 2 : 1;
-  __shared__ float sums[kActRows - 1][kSums][kActCols * 8];
+  __shared__ float sums[SUMS ? kActRows - 1 : 1][kSums][kActCols * 8];
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const int tc = threadIdx.x % kActCols, tr = threadIdx.x / kActCols;
@@ -670,75 +672,95 @@ __global__ void __launch_bounds__(kActCols * kActRows) act_backward_kernel(const
   const T* dy = static_cast<const T*>(a.dy) + c;
   const T* pre0 = static_cast<const T*>(a.pre[0]) + c;
   const T* pre1 = static_cast<const T*>(a.pre[1]) + c;
-  float s0[8] = {}, s1[8] = {};
+  [[maybe_unused]] float s0[8] = {}, s1[8] = {};
   with_act(a.act, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
     constexpr bool kReadsPre = GATED || ACT != GLQ_ACT_NONE;
-    for (long long r = lo; r < hi; r += 2 * kActRows) {
-      uint4 g[2], z[2], u[2];
+    struct Row {
+      uint4 g, z, u;
+    };
+    auto request = [&](long long row, Row& x) {
+      if (row < hi) {
+        x.g = load8_raw(dy + row * a.ld_dy, a.align_dy, valid);
+        if (kReadsPre) x.z = load8_raw(pre0 + row * a.ld_pre, a.align_pre, valid);
+        if (GATED) x.u = load8_raw(pre1 + row * a.ld_pre, a.align_pre, valid);
+      }
+    };
+    auto work = [&](long long row, const Row& x) {
+      const uint32_t gw[4] = {x.g.x, x.g.y, x.g.z, x.g.w};
+      const uint32_t zw[4] = {x.z.x, x.z.y, x.z.z, x.z.w};
+      const uint32_t uw[4] = {x.u.x, x.u.y, x.u.z, x.u.w};
+      uint32_t d0[4], d1[4];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const long long row = r + k * kActRows;
-        if (row < hi) {
-          g[k] = load8_raw(dy + row * a.ld_dy, a.align_dy, valid);
-          if (kReadsPre) z[k] = load8_raw(pre0 + row * a.ld_pre, a.align_pre, valid);
-          if (GATED) u[k] = load8_raw(pre1 + row * a.ld_pre, a.align_pre, valid);
+      for (int i = 0; i < 4; ++i) {  // elements past the row's end are zeros: so are their products
+        const float2 g = Elem16<T>::to_f2(gw[i]);
+        float2 value = {0.0f, 0.0f}, slope = {1.0f, 1.0f};
+        if (kReadsPre) {
+          const float2 z = Elem16<T>::to_f2(zw[i]);
+          act_grad_f<ACT>(z.x, &value.x, &slope.x);
+          act_grad_f<ACT>(z.y, &value.y, &slope.y);
+        }
+        float2 p = {g.x * slope.x, g.y * slope.y};
+        if (GATED) {
+          const float2 u = Elem16<T>::to_f2(uw[i]);
+          p = {p.x * u.x, p.y * u.y};
+          const float2 q = {g.x * value.x, g.y * value.y};
+          d1[i] = Elem16<T>::from_f2(q.x, q.y);
+          if (SUMS) {
+            s1[2 * i] += q.x;
+            s1[2 * i + 1] += q.y;
+          }
+        }
+        d0[i] = Elem16<T>::from_f2(p.x, p.y);
+        if (SUMS) {
+          s0[2 * i] += p.x;
+          s0[2 * i + 1] += p.y;
         }
       }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const long long row = r + k * kActRows;
-        if (row >= hi) break;
-        const uint32_t gw[4] = {g[k].x, g[k].y, g[k].z, g[k].w};
-        const uint32_t zw[4] = {z[k].x, z[k].y, z[k].z, z[k].w};
-        const uint32_t uw[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
-        float d0[8], d1[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // elements past the row's end are zeros: so are their products
-          const float2 gf = Elem16<T>::to_f2(gw[i / 2]);
-          const float gv = i & 1 ? gf.y : gf.x;
-          float value = 0.0f, slope = 1.0f;
-          if (kReadsPre) {
-            const float2 zf = Elem16<T>::to_f2(zw[i / 2]);
-            act_grad_f<ACT>(i & 1 ? zf.y : zf.x, &value, &slope);
-          }
-          if (GATED) {
-            const float2 uf = Elem16<T>::to_f2(uw[i / 2]);
-            d0[i] = gv * (i & 1 ? uf.y : uf.x) * slope;
-            d1[i] = gv * value;
-            s1[i] += d1[i];
-          } else {
-            d0[i] = gv * slope;
-          }
-          s0[i] += d0[i];
+      if (a.dz[0] != nullptr) {  // null: column sums only
+        store8_raw(static_cast<T*>(a.dz[0]) + row * a.ld_dz + c, a.align_dz, valid,
+                   make_uint4(d0[0], d0[1], d0[2], d0[3]));
+        if (GATED) {
+          store8_raw(static_cast<T*>(a.dz[1]) + row * a.ld_dz + c, a.align_dz, valid,
+                     make_uint4(d1[0], d1[1], d1[2], d1[3]));
         }
-        if (a.dz[0] != nullptr) {  // null: column sums only
-          store8(static_cast<T*>(a.dz[0]) + row * a.ld_dz + c, a.align_dz, valid, d0);
-          if (GATED) store8(static_cast<T*>(a.dz[1]) + row * a.ld_dz + c, a.align_dz, valid, d1);
-        }
+      }
+    };
+    Row even, odd;
+    request(lo, even);
+    request(lo + kActRows, odd);
+    for (long long r = lo; r < hi; r += 2 * kActRows) {
+      const Row now = even;
+      request(r + 2 * kActRows, even);
+      work(r, now);
+      if (r + kActRows < hi) {
+        const Row then = odd;
+        request(r + 3 * kActRows, odd);
+        work(r + kActRows, then);
       }
     }
   });
-  if (a.part == nullptr) return;
-  if (tr > 0) {
+  if constexpr (SUMS) {
+    if (tr > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sums[tr - 1][0][tc * 8 + i] = s0[i];
-      if (GATED) sums[tr - 1][kSums - 1][tc * 8 + i] = s1[i];
-    }
-  }
-  __syncthreads();
-  if (tr == 0 && live) {
-    float* part = a.part + static_cast<long long>(blockIdx.y) * kSums * a.part_cols + c;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll
-      for (int q = 0; q < kActRows - 1; ++q) {
-        s0[i] += sums[q][0][tc * 8 + i];
-        if (GATED) s1[i] += sums[q][kSums - 1][tc * 8 + i];
+      for (int i = 0; i < 8; ++i) {
+        sums[tr - 1][0][tc * 8 + i] = s0[i];
+        if (GATED) sums[tr - 1][kSums - 1][tc * 8 + i] = s1[i];
       }
-      part[i] = s0[i];
-      if (GATED) part[a.part_cols + i] = s1[i];
+    }
+    __syncthreads();
+    if (tr == 0 && live) {
+      float* part = a.part + static_cast<long long>(blockIdx.y) * kSums * a.part_cols + c;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int q = 0; q < kActRows - 1; ++q) {
+          s0[i] += sums[q][0][tc * 8 + i];
+          if (GATED) s1[i] += sums[q][kSums - 1][tc * 8 + i];
+        }
+        part[i] = s0[i];
+        if (GATED) part[a.part_cols + i] = s1[i];
+      }
     }
   }
 }
@@ -908,8 +930,14 @@ cudaError_t act_backward_typed(const ActBackwardArgs& a, bool gated, void* const
                                unsigned int flags, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>((a.cols + kActCols * 8 - 1) / (kActCols * 8)), static_cast<unsigned>(n_strips));
   constexpr int kThreads = kActCols * kActRows;
-  cudaError_t e = gated ? launch(act_backward_kernel<T, true>, grid, kThreads, 0, a, flags, s)
-                        : launch(act_backward_kernel<T, false>, grid, kThreads, 0, a, flags, s);
+  cudaError_t e;
+  if (a.part != nullptr) {
+    e = gated ? launch(act_backward_kernel<T, true, true>, grid, kThreads, 0, a, flags, s)
+              : launch(act_backward_kernel<T, false, true>, grid, kThreads, 0, a, flags, s);
+  } else {
+    e = gated ? launch(act_backward_kernel<T, true, false>, grid, kThreads, 0, a, flags, s)
+              : launch(act_backward_kernel<T, false, false>, grid, kThreads, 0, a, flags, s);
+  }
   if (e != cudaSuccess || a.part == nullptr) return e;
   ColumnSumArgs c = {};
   c.part = a.part;
