@@ -357,8 +357,8 @@ enum glq_activation {
  *     operands are first copied into the workspace.
  *   - workspace: device memory of at least the matching *_workspace_bytes()
  *     bytes, 256-byte aligned (GLQ_ERR_WORKSPACE otherwise; NULL when that is
- *     0).  It holds nothing between calls: calls that may overlap need
- *     workspaces of their own.
+ *     0; the size is that of the current device).  It holds nothing between
+ *     calls: calls that may overlap need workspaces of their own.
  *   - Optional pointers may be NULL; an output that is NULL is not computed.
  *   - Outputs must not overlap inputs or each other, except that Y of
  *     glq_fused_linear may be its residual (same address and row stride).
