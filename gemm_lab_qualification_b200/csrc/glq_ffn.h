@@ -52,8 +52,8 @@ struct Product {
   unsigned int flags = 0;  // glq_flags
 };
 
-// Largest token count of the skinny kernel's one-pass tiles.
-constexpr int kSkinnyTokens = 128;
+// Largest token tile of the skinny kernel.
+constexpr int kSkinnyTokens = 192;
 
 // How a launch of the pair kernel is scheduled (see glq_pair.cu).
 struct PairPlan {

@@ -873,12 +873,16 @@ int64_t strips(int64_t rows, int64_t cols, int sm_count) {
   return std::max<int64_t>(1, std::min<int64_t>(rows, std::min<int64_t>(4096, (int64_t{sm_count} * 4 + across - 1) / across)));
 }
 
-// Row strips of act_backward_kernel: eight blocks per SM, each of at least
-// the rows that its threads take at a time.
-int64_t act_strips(int64_t rows, int64_t cols, int sm_count) {
+// Row strips of act_backward_kernel: one wave of blocks (three per SM, two
+// with the gated sums) if whole strips fill most of it, else a few; at least
+// the rows that a block's threads take in two steps each.
+int64_t act_strips(int64_t rows, int64_t cols, int64_t sums, int sm_count) {
   const int64_t across = (cols + kActCols * 8 - 1) / (kActCols * 8);
+  const int64_t wave = int64_t{sm_count} * (sums == 2 ? 2 : 3);
+  int64_t n = wave / across;
+  if (n * across * 5 < wave * 4) n = (4 * wave + across - 1) / across;
   const int64_t most = (rows + 2 * kActRows - 1) / (2 * kActRows);
-  return std::max<int64_t>(1, std::min<int64_t>(most, std::min<int64_t>(4096, (int64_t{sm_count} * 8 + across - 1) / across)));
+  return std::max<int64_t>(1, std::min<int64_t>(most, std::min<int64_t>(4096, n)));
 }
 
 template <typename T>
@@ -968,7 +972,7 @@ size_t norm_backward_partial_bytes(int64_t rows, int64_t cols, int sm_count) {
 
 size_t act_backward_partial_bytes(int64_t rows, int64_t cols, int sums, int sm_count) {
   if (rows <= 0 || cols <= 0) return 0;
-  return static_cast<size_t>(act_strips(rows, cols, sm_count) * sums * padded(cols)) * sizeof(float);
+  return static_cast<size_t>(act_strips(rows, cols, sums, sm_count) * sums * padded(cols)) * sizeof(float);
 }
 
 cudaError_t launch_norm(int dtype, NormArgs a, int sm_count, unsigned int flags, cudaStream_t s) {
@@ -995,7 +999,7 @@ cudaError_t launch_act_backward(int dtype, bool gated, ActBackwardArgs a, void* 
   a.align_pre = std::min(row_align(a.pre[0], a.ld_pre), row_align(a.pre[1], a.ld_pre));
   a.align_dz = std::min(row_align(a.dz[0], a.ld_dz), row_align(a.dz[1], a.ld_dz));
   a.part_cols = padded(a.cols);
-  const int64_t n = act_strips(a.rows, a.cols, sm_count);
+  const int64_t n = act_strips(a.rows, a.cols, a.part == nullptr ? 0 : gated ? 2 : 1, sm_count);
   return dtype == GLQ_DTYPE_BF16 ? act_backward_typed<__nv_bfloat16>(a, gated, dbias, n, flags, s)
                                  : act_backward_typed<__half>(a, gated, dbias, n, flags, s);
 }

@@ -4,7 +4,7 @@
 //   out[m, n] = epilogue(sum_k A[m, k] W[n, k]),  W = B^T
 //
 // Bound: the bytes of W, each read once.  So the weight rows fill the 128
-// lanes of the MMA's M dimension, the tokens are its N dimension (16..128),
+// lanes of the MMA's M dimension, the tokens are its N dimension (16..192),
 // and the work is spread so that every SM streams weights:
 //   * One CTA owns 128 weight rows x one token tile x one contiguous range of
 //     64-wide K blocks; two CTAs share an SM (about 100 KB of loads in flight
@@ -19,7 +19,7 @@
 //     copy per owner, completing on the owner's barrier (1 x 4096 x 4096: 9.3
 //     us when owners read them through distributed shared memory between two
 //     cluster barriers); the receive buffer of 128 tokens would cost the second
-//     CTA per SM, so those are read.
+//     CTA per SM, so those are read.  192 tokens take one CTA per SM.
 //   * The epilogue (bias, activation, product, residual) runs on those sums
 //     in FP32 with one rounding per output.
 // The same kernel computes the input gradient for few tokens (W MN-major, and
@@ -41,21 +41,24 @@ constexpr int kThreads = 256;
 constexpr int kRows = 128;  // weight rows per CTA
 constexpr uint32_t kMnBox = 64 * kBK * 2;
 constexpr uint32_t kTwoPerSm = 233472u / 2u - 1024u;
+constexpr uint32_t kOnePerSm = 232448u;
 
 template <int BT>
 struct SkinnyConfig {
   static constexpr uint32_t kWBytes = kRows * kBK * 2;
   static constexpr uint32_t kABytes = BT * kBK * 2;
   static constexpr uint32_t kStageBytes = kWBytes + kABytes;
-  static constexpr int kStages = BT == 16 ? 5 : BT == 32 ? 4 : 3;
+  // Two CTAs per SM up to 128 tokens, one beyond.
+  static constexpr int kPerSm = BT <= 128 ? 2 : 1;
+  static constexpr int kStages = BT == 16 || BT == 192 ? 5 : BT == 32 ? 4 : 3;
   static constexpr uint32_t kRing = kStages * kStageBytes;
   static constexpr bool kPush = BT <= 64;
   // Largest receive buffer: split - 1 partials of ceil(BT / 4 / split) groups.
   static constexpr uint32_t kReceive = !kPush ? 0 : BT <= 32 ? 7 * kRows * 16 : 7 * 2 * kRows * 16;
   static constexpr int kBars = 2 * kStages + 2;
   static constexpr uint32_t kSmem = 1024 + kRing + kReceive + kBars * 8 + 16;
-  static constexpr uint32_t kTmemCols = BT < 32 ? 32 : BT;
-  static_assert(kSmem <= kTwoPerSm, "two CTAs per SM");
+  static constexpr uint32_t kTmemCols = BT < 32 ? 32 : BT == 192 ? 256 : BT;
+  static_assert(kSmem <= (kPerSm == 2 ? kTwoPerSm : kOnePerSm), "shared memory");
   static_assert(kRows * BT * 4 <= kRing, "the partial tile reuses the ring");
 };
 
@@ -80,7 +83,7 @@ struct SkinnyArgs {
 };
 
 template <typename T, int BT, bool W_MN, bool GATED>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, SkinnyConfig<BT>::kPerSm)
     skinny_kernel(const __grid_constant__ SkinnyMaps maps, const __grid_constant__ SkinnyArgs args) {
   using Cfg = SkinnyConfig<BT>;
   using E = Elem16<T>;
@@ -441,13 +444,16 @@ cudaError_t launch_typed(const Product& p, int sm_count, unsigned int* err, cuda
   }
   const int64_t tiles_n = (p.n + kOutRows - 1) / kOutRows, tiles_m = (p.m + BT - 1) / BT;
   if (tiles_m > 65535 || tiles_n > 65535) return cudaErrorInvalidValue;
-  // As many K ranges as still fit two CTAs on every SM, each of at least four
-  // K blocks (a shorter range is all latency).  The receive buffer is sized for
-  // these counts; 3 fills the device where 2 leaves 40 % of it idle (32 x 11008
-  // x 4096: 19.2 us in 2 ranges, 17.8 in 3).
+  // As many K ranges as still run at once, each of at least four K blocks (a
+  // shorter range is all latency).  The receive buffer is sized for these
+  // counts; 3 fills the device where 2 leaves 40 % of it idle (32 x 11008 x
+  // 4096: 19.2 us in 2 ranges, 17.8 in 3).  Clusters of 8 stay inside a GPC:
+  // 33 of them run at once with two CTAs per SM, 15 with one.
+  const int64_t eights = int64_t{sm_count} * (Cfg::kPerSm == 2 ? 33 : 15) / 148;
   int split = 1;
   for (int q : {2, 3, 4, 8}) {
-    if (tiles_n * tiles_m * q <= 2 * sm_count && args.kb_total / q >= 4) split = q;
+    const int64_t tiles = tiles_n * tiles_m;
+    if ((q == 8 ? tiles <= eights : tiles * q <= Cfg::kPerSm * sm_count) && args.kb_total / q >= 4) split = q;
   }
   args.split = split;
 
@@ -484,7 +490,8 @@ cudaError_t launch_tokens(const Product& p, int sm_count, unsigned int* err, cud
   if (p.m <= 16) return launch_order<T, 16>(p, sm_count, err, s);
   if (p.m <= 32) return launch_order<T, 32>(p, sm_count, err, s);
   if (p.m <= 64) return launch_order<T, 64>(p, sm_count, err, s);
-  return launch_order<T, 128>(p, sm_count, err, s);
+  if (p.m <= 128 || p.k == 0) return launch_order<T, 128>(p, sm_count, err, s);
+  return launch_order<T, 192>(p, sm_count, err, s);
 }
 
 template <typename T, int BT>
@@ -504,6 +511,7 @@ cudaError_t set_attrs_all() {
   if (e == cudaSuccess) e = set_attrs<T, 32>();
   if (e == cudaSuccess) e = set_attrs<T, 64>();
   if (e == cudaSuccess) e = set_attrs<T, 128>();
+  if (e == cudaSuccess) e = set_attrs<T, 192>();
   return e;
 }
 

@@ -69,7 +69,7 @@ def d(t):
 SIZES = [(1, 64, 64), (1, 1000, 4096), (2, 31, 13), (3, 72, 40), (8, 136, 200), (16, 200, 1032), (17, 257, 131),
          (32, 1032, 520), (33, 40, 2056), (64, 128, 320), (65, 300, 72), (100, 8, 1), (127, 1, 64), (128, 520, 264),
          (129, 257, 65), (200, 384, 512), (256, 256, 64), (257, 136, 136), (300, 1000, 1000), (513, 264, 1544),
-         (600, 2056, 128), (1025, 65, 520)]
+         (600, 2056, 128), (1025, 65, 520), (160, 1000, 520), (192, 264, 1032), (193, 72, 200)]
 W_LAYOUTS = ["nk", "kn", "nk_padded", "kn_padded", "nk_offset", "strided"]
 A_LAYOUTS = ["plain", "padded", "odd", "transposed"]
 
