@@ -834,7 +834,7 @@ cudaError_t launch_typed(const Product* products, int count, const PairPlan& pla
   args.partials = static_cast<float*>(workspace);
   args.flags = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(workspace) + plan.runs * kSlotTile);
   args.epoch = next_epoch();
-  args.group_m = 16;
+  args.group_m = 8;
   args.act = p.act;
   args.residual = p.residual;
   args.ld_residual = p.ld_residual;
