@@ -84,6 +84,99 @@ __device__ __forceinline__ void store8(T* p, int align, int valid, const float (
                         Elem16<T>::from_f2(v[6], v[7])));
 }
 
+// Which columns of a row a thread of its group of G holds: in its vector j of 8
+// the pair i begins at column(j, i).  VEC (rows of whole 16-byte vectors): 8
+// consecutive columns.  Other rows: a warp's 256 columns of a vector are dealt
+// out in pairs, so that each of its loads and stores covers 128 bytes in a row
+// (consecutive columns there, 2 to 8 bytes at a time from 512 bytes: 8192 x
+// 4095 forward 117 us, backward 173 us; 61 and 111 so).
+template <int G, bool VEC>
+struct Columns {
+  int first;
+  __device__ __forceinline__ Columns() {
+    const int t = threadIdx.x % G;
+    first = VEC ? t * 8 : (t / 32) * 256 + (t % 32) * 2;
+  }
+  __device__ __forceinline__ int column(int j, int i) const { return first + j * G * 8 + (VEC ? 2 : 64) * i; }
+};
+
+// Loads and stores under a predicate instead of a branch: none waits for the
+// one before it.
+__device__ __forceinline__ uint32_t ld_u32_if(const void* p, bool on) {
+  uint32_t v;
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n mov.b32 %0, 0;\n @q ld.global.b32 %0, [%1];\n}"
+               : "=&r"(v) : "l"(p), "r"(static_cast<int>(on)));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_u16_if(const void* p, bool on) {
+  uint16_t v;
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n mov.b16 %0, 0;\n @q ld.global.b16 %0, [%1];\n}"
+               : "=&h"(v) : "l"(p), "r"(static_cast<int>(on)));
+  return v;
+}
+__device__ __forceinline__ void st_u32_if(void* p, bool on, uint32_t v) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q st.global.b32 [%0], %1;\n}"
+               :: "l"(p), "r"(v), "r"(static_cast<int>(on)) : "memory");
+}
+__device__ __forceinline__ void st_u16_if(void* p, bool on, uint32_t v) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q st.global.b16 [%0], %1;\n}"
+               :: "l"(p), "h"(static_cast<uint16_t>(v)), "r"(static_cast<int>(on)) : "memory");
+}
+
+__device__ __forceinline__ bool in_words(const void* row) { return (reinterpret_cast<uintptr_t>(row) & 3) == 0; }
+
+// The pairs of vectors first to first + V of a row (0 past its end), by whole
+// words where the row begins at one.
+template <typename T, int V, typename C>
+__device__ __forceinline__ void load_pairs(const T* row, const C& mine, int cols, uint4 (&out)[V], int first = 0) {
+  const bool words = in_words(row);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    uint32_t w[4];
+    if (words) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = mine.column(first + j, i);
+        w[i] = ld_u32_if(row + c, c + 1 < cols);
+      }
+      if (cols & 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = mine.column(first + j, i);
+          w[i] |= ld_u16_if(row + c, c + 1 == cols);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = mine.column(first + j, i);
+        w[i] = ld_u16_if(row + c, c < cols) | (ld_u16_if(row + c + 1, c + 1 < cols) << 16);
+      }
+    }
+    out[j] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <typename T, typename C>
+__device__ __forceinline__ void store_pairs(T* row, const C& mine, int cols, int j, const uint4& x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  if (in_words(row)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = mine.column(j, i);
+      st_u32_if(row + c, c + 1 < cols, w[i]);
+      st_u16_if(row + c, c + 1 == cols, w[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = mine.column(j, i);
+      st_u16_if(row + c, c < cols, w[i]);
+      st_u16_if(row + c + 1, c + 1 < cols, w[i] >> 16);
+    }
+  }
+}
+
 // Sum of N values over the G threads of a row.  Groups of more than a warp
 // join through red[2][G / 32][N], their own, behind the group's named barrier;
 // every thread adds the warps' sums in the same order.
@@ -215,7 +308,7 @@ __device__ __forceinline__ uint4 ld_smem_v4(uint32_t at) {
 // one (one row per block instead: 159 us at 16384 x 8192; rows by bulk copies
 // through shared memory: 123 us, the joins' latency then has too few groups
 // per SM to hide behind), and arithmetic is paired.  VEC: rows of whole
-// 16-byte vectors; other rows are read where they are used.
+// 16-byte vectors; other rows are held in pairs of columns (Columns).
 
 constexpr int kNormThreads = 256;
 
@@ -225,7 +318,7 @@ __global__ void __launch_bounds__(G < kNormThreads ? kNormThreads : G, G < 512 ?
   __shared__ float red[kGroups * 2 * (G / 32)];
   int phase = 0;
   const int group = threadIdx.x / G;
-  const int c0 = (threadIdx.x % G) * 8;
+  const Columns<G, VEC> mine;
   const int cols = a.cols;
   const float inv = 1.0f / static_cast<float>(cols);
   float* my_red = red + group * 2 * (G / 32);
@@ -236,14 +329,17 @@ __global__ void __launch_bounds__(G < kNormThreads ? kNormThreads : G, G < 512 ?
   const T* x = static_cast<const T*>(a.x);
   const long long step = static_cast<long long>(gridDim.x) * kGroups;
   long long r = static_cast<long long>(blockIdx.x) * kGroups + group;
-  uint4 next[VEC ? V : 1];
+  uint4 next[V];
   auto request = [&](long long row) {
+    const T* from = x + row * a.ld_x;
     if constexpr (VEC) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int c = c0 + j * G * 8;
-        next[j] = c < cols ? ptx::ldg_stream_v4(x + row * a.ld_x + c) : make_uint4(0, 0, 0, 0);
+        const int c = mine.column(j, 0);
+        next[j] = c < cols ? ptx::ldg_stream_v4(from + c) : make_uint4(0, 0, 0, 0);
       }
+    } else {
+      load_pairs(from, mine, cols, next);
     }
   };
   if (r < a.rows) request(r);
@@ -252,15 +348,7 @@ __global__ void __launch_bounds__(G < kNormThreads ? kNormThreads : G, G < 512 ?
     Two acc = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if constexpr (VEC) {
-        unpack<T>(next[j], v[j]);
-      } else {
-        const int c = c0 + j * G * 8;
-        float f[8];
-        load8(x + r * a.ld_x + c, a.align, cols - c, f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[j][i] = two(f[2 * i], f[2 * i + 1]);
-      }
+      unpack<T>(next[j], v[j]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc = add2(acc, v[j][i]);
     }
@@ -272,12 +360,12 @@ __global__ void __launch_bounds__(G < kNormThreads ? kNormThreads : G, G < 512 ?
     acc = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = c0 + j * G * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        const int c = mine.column(j, VEC ? 0 : i);
         v[j][i] = add2(v[j][i], minus_mean);
-        if (!VEC && c + 2 * i + 1 >= cols) {  // past the end, or the last of an odd number
-          v[j][i] = two(c + 2 * i < cols ? halves(v[j][i]).x : 0.0f, 0.0f);
+        if (!VEC && c + 1 >= cols) {  // past the end, or the last of an odd number
+          v[j][i] = two(c < cols ? halves(v[j][i]).x : 0.0f, 0.0f);
         }
         if (!VEC || c < cols) acc = fma2(v[j][i], v[j][i], acc);
       }
@@ -289,11 +377,11 @@ __global__ void __launch_bounds__(G < kNormThreads ? kNormThreads : G, G < 512 ?
     T* y = static_cast<T*>(a.y) + r * a.ld_y;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = c0 + j * G * 8;
-      if (c >= cols) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[j][i] = mul2(v[j][i], scale);
       if constexpr (VEC) {  // (align_w is 16)
+        const int c = mine.column(j, 0);
+        if (c >= cols) continue;
         Two w[4];
         if (weight != nullptr) {
           unpack<T>(*reinterpret_cast<const uint4*>(weight + c), w);
@@ -307,26 +395,24 @@ __global__ void __launch_bounds__(G < kNormThreads ? kNormThreads : G, G < 512 ?
         }
         *reinterpret_cast<uint4*>(y + c) = pack<T>(v[j]);
       } else {
-        float f[8], w[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f[2 * i] = halves(v[j][i]).x;
-          f[2 * i + 1] = halves(v[j][i]).y;
-        }
+        uint4 raw[1];
+        Two w[4];
         if (weight != nullptr) {
-          load8(weight + c, a.align_w, cols - c, w);
+          load_pairs(weight, mine, cols, raw, j);
+          unpack<T>(raw[0], w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] *= w[i];
+          for (int i = 0; i < 4; ++i) v[j][i] = mul2(v[j][i], w[i]);
         }
         if (bias != nullptr) {
-          load8(bias + c, a.align_w, cols - c, w);
+          load_pairs(bias, mine, cols, raw, j);
+          unpack<T>(raw[0], w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] += w[i];
+          for (int i = 0; i < 4; ++i) v[j][i] = add2(v[j][i], w[i]);
         }
-        store8(y + c, a.align, cols - c, f);
+        store_pairs(y, mine, cols, j, pack<T>(v[j]));
       }
     }
-    if (c0 == 0 && a.mean != nullptr) {
+    if (threadIdx.x % G == 0 && a.mean != nullptr) {
       a.mean[r] = mean;
       a.rstd[r] = rstd;
     }
@@ -405,7 +491,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
   extern __shared__ __align__(128) uint8_t dyn_smem[];  // weight, rings; at the end: float [groups][2][part_cols]
   int phase = 0;
   const int group = threadIdx.x / G;
-  const int c0 = (threadIdx.x % G) * 8;
+  const Columns<G, VEC> mine;
+  const bool leads = threadIdx.x % G == 0;
   const int cols = a.cols;
   float* weight = reinterpret_cast<float*>(dyn_smem);
   const float inv = 1.0f / static_cast<float>(cols);
@@ -427,7 +514,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
   ring.err = a.err;
   ring.policy = ptx::policy_evict_first();
   auto start = [&](long long row) { ring.start({x + row * a.ld_x, dy + row * a.ld_dy}); };
-  if (VEC && c0 == 0) {
+  if (VEC && leads) {
     for (int i = 0; i < kStages && r + i * step < a.rows; ++i) start(r + i * step);
   }
   float next_mean = 0.0f, next_rstd = 0.0f;
@@ -453,27 +540,40 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
       next_rstd = a.rstd[r + step];
     }
     [[maybe_unused]] const uint32_t slot = VEC ? ring.wait() : 0u;
+    [[maybe_unused]] uint4 x_raw[VEC ? 1 : V], dy_raw[VEC ? 1 : V];
+    if constexpr (!VEC) {
+      load_pairs(x + r * a.ld_x, mine, cols, x_raw);
+      load_pairs(dy + r * a.ld_dy, mine, cols, dy_raw);
+    }
     // x and dy of vector j (0 past the row's end).
     auto at = [&](int j, Two(&xv)[4], Two(&gv)[4]) {
-      const int c = c0 + j * G * 8;
       if constexpr (VEC) {
+        const int c = mine.column(j, 0);
         unpack<T>(ld_smem_v4(slot + 2 * c), xv);
         unpack<T>(ld_smem_v4(slot + ring.row_bytes + 2 * c), gv);
       } else {
-        unpack<T>(load8_raw(x + r * a.ld_x + c, a.align, cols - c), xv);
-        unpack<T>(load8_raw(dy + r * a.ld_dy + c, a.align, cols - c), gv);
+        unpack<T>(x_raw[j], xv);
+        unpack<T>(dy_raw[j], gv);
       }
     };
     auto weights = [&](int j, Two(&w)[4]) {
-      const ulonglong2* p = reinterpret_cast<const ulonglong2*>(weight + c0 + j * G * 8);
-      const ulonglong2 lo = p[0], hi = p[1];
-      w[0] = lo.x, w[1] = lo.y, w[2] = hi.x, w[3] = hi.y;
+      if constexpr (VEC) {
+        const ulonglong2* p = reinterpret_cast<const ulonglong2*>(weight + mine.column(j, 0));
+        const ulonglong2 lo = p[0], hi = p[1];
+        w[0] = lo.x, w[1] = lo.y, w[2] = hi.x, w[3] = hi.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = mine.column(j, i);
+          w[i] = c < cols ? *reinterpret_cast<const Two*>(weight + c) : 0;  // (part_cols is even)
+        }
+      }
     };
     const Two rstd2 = two(rstd, rstd), shift2 = two(shift, shift);
     Two s0 = 0, s1 = 0;  // sums of dy w xhat and of dy w
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (c0 + j * G * 8 >= cols) continue;
+      if (VEC && mine.column(j, 0) >= cols) continue;
       Two xv[4], g[4], w[4];
       at(j, xv, g);
       weights(j, w);
@@ -490,7 +590,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
     row_sum<G>(sum, my_red, phase, group);
     // Past this join the whole group is done with the row before this one:
     // its slot takes the row kStages - 1 ahead.
-    if (VEC && c0 == 0 && ring.use > 1 && r + (kStages - 1) * step < a.rows) start(r + (kStages - 1) * step);
+    if (VEC && leads && ring.use > 1 && r + (kStages - 1) * step < a.rows) start(r + (kStages - 1) * step);
     // dx = (rstd w) dy - rstd mean(g xhat) xhat - rstd mean(g)
     const float k1 = -rstd * (sum[0] * inv), k2 = -rstd * (sum[1] * inv);
     const float level1 = fmaf(shift, k1, k2);
@@ -498,17 +598,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
     T* dx = static_cast<T*>(a.dx) + r * a.ld_dx;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = c0 + j * G * 8;
-      if (c >= cols) continue;
+      if (VEC && mine.column(j, 0) >= cols) continue;
       Two xv[4], g[4], w[4];
       at(j, xv, g);
       weights(j, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) g[i] = fma2(g[i], mul2(w[i], rstd2), fma2(xv[i], slope, level));
+      const uint4 raw = pack<T>(g);
       if constexpr (VEC) {
-        *reinterpret_cast<uint4*>(dx + c) = pack<T>(g);
+        *reinterpret_cast<uint4*>(dx + mine.column(j, 0)) = raw;
       } else {
-        store8_raw(dx + c, a.align, cols - c, pack<T>(g));
+        store_pairs(dx, mine, cols, j, raw);
       }
     }
   }
@@ -521,12 +621,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
   float* to = kGroups > 1 ? joined + static_cast<size_t>(group) * 2 * a.part_cols : part;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int c = c0 + j * G * 8;
-    if (c >= cols) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // part_cols is a multiple of 8
-      *reinterpret_cast<Two*>(to + c + 2 * i) = dw[j][i];
-      *reinterpret_cast<Two*>(to + a.part_cols + c + 2 * i) = db[j][i];
+      const int c = mine.column(j, i);
+      if (c >= a.part_cols) continue;
+      *reinterpret_cast<Two*>(to + c) = dw[j][i];
+      *reinterpret_cast<Two*>(to + a.part_cols + c) = db[j][i];
     }
   }
   if (kGroups > 1) {
@@ -817,27 +917,37 @@ cudaError_t norm_by_columns(const NormArgs& a, int grid, unsigned int flags, cud
   }
 }
 
-template <typename T, int G, int V>
+template <typename T, int G, int V, bool VEC>
 cudaError_t launch_rows_backward(const NormBackwardArgs& a, int grid, unsigned int flags, cudaStream_t s) {
   constexpr int kGroups = kRowThreads / G;
   // Weight and rings (at most 224 KB), then the groups' sums (at most 128 KB).
   const size_t one = static_cast<size_t>(a.part_cols) * sizeof(float);
-  const size_t ring = a.vec ? static_cast<size_t>(kGroups) * kBackwardStages<G> * 2 * a.cols * 2 : 0;
+  const size_t ring = VEC ? static_cast<size_t>(kGroups) * kBackwardStages<G> * 2 * a.cols * 2 : 0;
   const size_t smem = std::max(one + ring, kGroups > 1 ? kGroups * 2 * one : 0);
-  return a.vec ? launch(norm_backward_kernel<T, G, V, true>, dim3(grid), kRowThreads, smem, a, flags, s)
-               : launch(norm_backward_kernel<T, G, V, false>, dim3(grid), kRowThreads, smem, a, flags, s);
+  return launch(norm_backward_kernel<T, G, V, VEC>, dim3(grid), kRowThreads, smem, a, flags, s);
 }
 
 template <typename T>
 cudaError_t norm_backward_by_columns(const NormBackwardArgs& a, int grid, unsigned int flags, cudaStream_t s) {
-  if (a.cols <= 256) return launch_rows_backward<T, 32, 1>(a, grid, flags, s);
-  if (a.cols <= 512) return launch_rows_backward<T, 32, 2>(a, grid, flags, s);
+  if (a.cols <= 256) return a.vec ? launch_rows_backward<T, 32, 1, true>(a, grid, flags, s)
+                                : launch_rows_backward<T, 32, 1, false>(a, grid, flags, s);
+  if (a.cols <= 512) return a.vec ? launch_rows_backward<T, 32, 2, true>(a, grid, flags, s)
+                                : launch_rows_backward<T, 32, 2, false>(a, grid, flags, s);
+  if (!a.vec) {  // a row waits in registers: half of it per thread where a block is enough
+    switch (group_threads(a.cols)) {
+      case 32: return launch_rows_backward<T, 64, 2, false>(a, grid, flags, s);
+      case 64: return launch_rows_backward<T, 128, 2, false>(a, grid, flags, s);
+      case 128: return launch_rows_backward<T, 256, 2, false>(a, grid, flags, s);
+      case 256: return launch_rows_backward<T, 512, 2, false>(a, grid, flags, s);
+      default: return launch_rows_backward<T, 512, 4, false>(a, grid, flags, s);
+    }
+  }
   switch (group_threads(a.cols)) {
-    case 32: return launch_rows_backward<T, 32, 4>(a, grid, flags, s);
-    case 64: return launch_rows_backward<T, 64, 4>(a, grid, flags, s);
-    case 128: return launch_rows_backward<T, 128, 4>(a, grid, flags, s);
-    case 256: return launch_rows_backward<T, 256, 4>(a, grid, flags, s);
-    default: return launch_rows_backward<T, 512, 4>(a, grid, flags, s);
+    case 32: return launch_rows_backward<T, 32, 4, true>(a, grid, flags, s);
+    case 64: return launch_rows_backward<T, 64, 4, true>(a, grid, flags, s);
+    case 128: return launch_rows_backward<T, 128, 4, true>(a, grid, flags, s);
+    case 256: return launch_rows_backward<T, 256, 4, true>(a, grid, flags, s);
+    default: return launch_rows_backward<T, 512, 4, true>(a, grid, flags, s);
   }
 }
 
@@ -848,22 +958,28 @@ int64_t backward_blocks(int64_t rows, int64_t cols, int sm_count) {
   return std::min<int64_t>((rows + at_a_time - 1) / at_a_time, sm_count);
 }
 
-template <typename T, int G, int V>
+template <typename T, int G, int V, bool VEC>
 cudaError_t set_attr() {
-  constexpr cudaFuncAttribute kAttr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  const cudaError_t e = cudaFuncSetAttribute(norm_backward_kernel<T, G, V, true>, kAttr, 229376);
-  return e != cudaSuccess ? e : cudaFuncSetAttribute(norm_backward_kernel<T, G, V, false>, kAttr, 131072);
+  return cudaFuncSetAttribute(norm_backward_kernel<T, G, V, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              VEC ? 229376 : 131072);
 }
 
 template <typename T>
 cudaError_t set_attrs() {
-  cudaError_t e = set_attr<T, 32, 1>();
-  if (e == cudaSuccess) e = set_attr<T, 32, 2>();
-  if (e == cudaSuccess) e = set_attr<T, 32, 4>();
-  if (e == cudaSuccess) e = set_attr<T, 64, 4>();
-  if (e == cudaSuccess) e = set_attr<T, 128, 4>();
-  if (e == cudaSuccess) e = set_attr<T, 256, 4>();
-  if (e == cudaSuccess) e = set_attr<T, 512, 4>();
+  cudaError_t e = set_attr<T, 32, 1, true>();
+  if (e == cudaSuccess) e = set_attr<T, 32, 2, true>();
+  if (e == cudaSuccess) e = set_attr<T, 32, 4, true>();
+  if (e == cudaSuccess) e = set_attr<T, 64, 4, true>();
+  if (e == cudaSuccess) e = set_attr<T, 128, 4, true>();
+  if (e == cudaSuccess) e = set_attr<T, 256, 4, true>();
+  if (e == cudaSuccess) e = set_attr<T, 512, 4, true>();
+  if (e == cudaSuccess) e = set_attr<T, 32, 1, false>();
+  if (e == cudaSuccess) e = set_attr<T, 32, 2, false>();
+  if (e == cudaSuccess) e = set_attr<T, 64, 2, false>();
+  if (e == cudaSuccess) e = set_attr<T, 128, 2, false>();
+  if (e == cudaSuccess) e = set_attr<T, 256, 2, false>();
+  if (e == cudaSuccess) e = set_attr<T, 512, 2, false>();
+  if (e == cudaSuccess) e = set_attr<T, 512, 4, false>();
   return e;
 }
 

@@ -282,7 +282,9 @@ def test_non_finite_rows_stay_in_their_rows(m):
 
 
 NORM_SIZES = [(1, 1), (1, 8), (3, 33), (5, 256), (9, 264), (4, 512), (130, 520), (7, 1024), (6, 1032), (300, 2048),
-              (33, 2050), (1, 4096), (700, 4096), (5, 4104), (150, 8192), (6, 8200), (300, 16384), (3, 16392), (2, 20001)]
+              (33, 2050), (1, 4096), (700, 4096), (5, 4104), (150, 8192), (6, 8200), (300, 16384), (3, 16392), (2, 20001),
+              (958, 111), (40, 257), (7, 513), (300, 1001), (9, 1030), (1200, 2047), (40, 4095), (160, 8190), (5, 12001),
+              (4, 16383)]
 
 
 @pytest.mark.parametrize("i,size", list(enumerate(NORM_SIZES)), ids=[f"m{m}-n{n}" for m, n in NORM_SIZES])
