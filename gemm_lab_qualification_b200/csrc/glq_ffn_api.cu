@@ -42,7 +42,7 @@ struct Matrix {
 
 struct Copy {
   Matrix from;
-  void* to = nullptr;  // rows at repack_pitch(cols)
+  void* to = nullptr;  // rows at sector_pitch(cols)
 };
 
 struct Copies {
@@ -63,25 +63,46 @@ Matrix transposed(const Matrix& m) { return {m.ptr, m.cols, m.rows, m.cs, m.rs};
 
 enum class Major { kAny, kK, kMn };
 
-// m as an operand with m.cols the contraction.
-Operand operand(const Matrix& m, Major want, Arena* arena, Copies* copies) {
-  if (want != Major::kMn && row_addressable(m)) return {m.ptr, row_pitch(m), true};
+// Rows that begin at multiples of 16 bytes but not of 32 load at two thirds of
+// the rate: the TMA splits their 32-byte sectors.  One such operand slows the
+// pair kernel by an eighth, two by almost a half (512 tokens through 22528 x
+// 7104: 122 us; pitch of A, of B, of both off by 16 bytes: 146, 134, 175; 2048
+// tokens: 413, and 499, 481, 639), which a copy of the smaller one can be worth.
+constexpr double kOffSector[3] = {1.0, 1.12, 1.45};
+int64_t sector_pitch(int64_t cols) { return (cols + 15) / 16 * 16; }
+bool off_sector(const Matrix& m) {
+  const int64_t pitch = row_addressable(m) ? row_pitch(m) : row_addressable(transposed(m)) ? row_pitch(transposed(m)) : 0;
+  return !aligned(m.ptr, 32) || pitch % 16 != 0;
+}
+// Estimated times in us: a launch and the bytes both ways at 5.5 TB/s; a
+// product at 1.5 PFLOP/s.
+double copy_us(const Matrix& m) { return 2.5 + static_cast<double>(m.rows * m.cols * 2 * kEsz) / 5.5e6; }
+double product_us(int64_t m, int64_t n, int64_t k) {
+  return 2.0 * static_cast<double>(m) * static_cast<double>(n) * static_cast<double>(k) / 1.5e9;
+}
+
+// m as an operand with m.cols the contraction; `copy`: one whose rows can be
+// read as they are is copied all the same.
+Operand operand(const Matrix& m, Major want, Arena* arena, Copies* copies, bool copy = false) {
   const Matrix t = transposed(m);
-  if (want != Major::kK && row_addressable(t)) return {m.ptr, row_pitch(t), false};
+  const bool k_rows = want != Major::kMn && row_addressable(m), mn_rows = want != Major::kK && row_addressable(t);
+  if (!copy && k_rows) return {m.ptr, row_pitch(m), true};
+  if (!copy && mn_rows) return {m.ptr, row_pitch(t), false};
   // Copied in the order that reads it along its contiguous dimension if the
   // caller of this function leaves the choice.
   const bool mn = want == Major::kMn || (want == Major::kAny && m.cs != 1 && m.rs == 1);
   const Matrix from = mn ? t : m;
-  void* to = arena->take(static_cast<size_t>(from.rows) * repack_pitch(from.cols) * kEsz);
+  const int64_t pitch = sector_pitch(from.cols);
+  void* to = arena->take(static_cast<size_t>(from.rows) * pitch * kEsz);
   copies->list[copies->count].from = from;
   copies->list[copies->count++].to = to;
-  return {to, repack_pitch(from.cols), !mn};
+  return {to, pitch, !mn};
 }
 
 cudaError_t run_copies(const Copies& c, int sm_count, cudaStream_t s) {
   for (int i = 0; i < c.count; ++i) {
     const Matrix& f = c.list[i].from;
-    const cudaError_t e = launch_repack(f.ptr, f.rows, f.cols, f.rs, f.cs, c.list[i].to, sm_count, s);
+    const cudaError_t e = launch_repack(f.ptr, f.rows, f.cols, f.rs, f.cs, c.list[i].to, sm_count, s, sector_pitch(f.cols));
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -173,9 +194,24 @@ struct ForwardPlan {
 ForwardPlan plan_forward(Product* p, const Matrix& a, const Matrix& b0, const Matrix* b1, int sm_count,
                          Arena* arena) {
   ForwardPlan plan;
-  p->a[0] = operand(a, Major::kK, arena, &plan.copies);
-  p->b[0] = operand(b0, Major::kAny, arena, &plan.copies);
-  if (b1 != nullptr) p->b[1] = operand(*b1, p->b[0].k_major ? Major::kK : Major::kMn, arena, &plan.copies);
+  bool copy_a = false, copy_b = false;
+  p->a[0].k_major = true;
+  if (!is_skinny(*p, sm_count)) {
+    const int weights = b1 != nullptr ? 2 : 1;
+    const bool off_a = off_sector(a), off_b = off_sector(b0) || (b1 != nullptr && off_sector(*b1));
+    const double us = product_us(p->m, weights * p->n, p->k);
+    double best = us * kOffSector[off_a + off_b];
+    for (int c = 1; c < 4; ++c) {
+      const bool ca = (c & 1) != 0, cb = (c & 2) != 0;
+      if ((ca && !off_a) || (cb && !off_b)) continue;
+      const double t = us * kOffSector[(off_a && !ca) + (off_b && !cb)] + (ca ? copy_us(a) : 0.0) +
+                       (cb ? weights * copy_us(b0) : 0.0);
+      if (t < best) best = t, copy_a = ca, copy_b = cb;
+    }
+  }
+  p->a[0] = operand(a, Major::kK, arena, &plan.copies, copy_a);
+  p->b[0] = operand(b0, Major::kAny, arena, &plan.copies, copy_b);
+  if (b1 != nullptr) p->b[1] = operand(*b1, p->b[0].k_major ? Major::kK : Major::kMn, arena, &plan.copies, copy_b);
   plan.workspace = arena->take(product_workspace(*p, sm_count));
   return plan;
 }
@@ -250,7 +286,7 @@ BackwardPlan plan_backward(const Backward& q, unsigned int flags, int sm_count, 
   p.make_dz = products && (q.gated || q.act != GLQ_ACT_NONE || !row_addressable(dy));
   if (p.make_dz) {
     for (int i = 0; i < pair; ++i) {
-      const int64_t pitch = repack_pitch(q.n);
+      const int64_t pitch = sector_pitch(q.n);
       p.dz[i] = {arena->take(static_cast<size_t>(q.m) * pitch * kEsz), pitch, true};
     }
   } else {
@@ -331,7 +367,7 @@ int run_backward(const Backward& q, unsigned int flags, void* workspace, size_t 
     a.dy = q.dy;
     a.ld_dy = q.ld_dy;
     a.ld_pre = q.ld_pre;
-    a.ld_dz = repack_pitch(q.n);
+    a.ld_dz = sector_pitch(q.n);
     a.rows = q.m;
     a.cols = static_cast<int>(q.n);
     a.act = q.act;

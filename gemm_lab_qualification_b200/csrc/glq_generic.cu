@@ -404,9 +404,9 @@ cudaError_t launch_small(const Problem& p, cudaStream_t s) {
 }
 
 cudaError_t launch_repack(const void* src, int64_t rows, int64_t cols, int64_t rs, int64_t cs, void* dst,
-                          int sm_count, cudaStream_t s) {
+                          int sm_count, cudaStream_t s, int64_t pitch) {
   if (rows <= 0 || cols <= 0) return cudaSuccess;
-  const long long pitch_chunks = repack_pitch(cols) / 8;
+  const long long pitch_chunks = (pitch > 0 ? pitch : repack_pitch(cols)) / 8;
   const long long sms = sm_count > 0 ? sm_count : 148;
   if (cs == 1 || cols == 1) {
     const long long chunks = rows * pitch_chunks;

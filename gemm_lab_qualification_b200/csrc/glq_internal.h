@@ -229,10 +229,10 @@ cudaError_t launch_small(const Problem& p, cudaStream_t s);
 // boundaries.
 inline int64_t repack_pitch(int64_t cols) { return (cols + 7) / 8 * 8; }
 // Copies rows x cols 2-byte elements, element (r, c) at src + r*rs + c*cs
-// (any alignment), into dst (16-byte aligned) with row pitch
-// repack_pitch(cols); the pad columns are written as zero.
+// (any alignment), into dst (16-byte aligned) with row pitch `pitch` (a
+// multiple of 8; 0: repack_pitch(cols)); the pad columns are written as zero.
 cudaError_t launch_repack(const void* src, int64_t rows, int64_t cols, int64_t rs, int64_t cs, void* dst,
-                          int sm_count, cudaStream_t s);
+                          int sm_count, cudaStream_t s, int64_t pitch = 0);
 // Returns cudaErrorNotSupported-style codes through `status` for TMA encode
 // problems (GLQ_ERR_CUDA).
 // gather: null for a plain call (the output is p.y only).

@@ -111,6 +111,11 @@ def test_workspace_sizes():
     # A of 4 rows, W of 64 rows, 61 columns each in 64-element pitches, in 256-byte steps.
     assert lib.glq_fused_linear_workspace_bytes(0, P, 61, 1, P, 1, 61, 4, 64, 61) == 4 * 128 + 64 * 128
     assert lib.glq_fused_linear_workspace_bytes(0, P, 64, 1, P, 1, 61, 0, 64, 61) == 0
+    # Rows at odd multiples of 16 bytes: the smaller operand is copied to whole sectors where that pays.
+    whole, off = (lib.glq_fused_linear_workspace_bytes(0, P, ld, 1, P, 1, ld, 512, 8192, 4104) for ld in (4112, 4104))
+    assert off - whole == 512 * 4112 * 2
+    whole, off = (lib.glq_fused_linear_workspace_bytes(0, P, ld, 1, P, 1, ld, 512, 256, 136) for ld in (144, 136))
+    assert off == whole
     # The gated pair copies an up weight of another order than the gate's.
     assert lib.glq_gated_linear_workspace_bytes(0, P, 64, 1, P, 1, 64, P, 64, 1, 4, 64, 64) == 64 * 128
     assert lib.glq_gated_linear_workspace_bytes(0, P, 64, 1, P, 64, 1, P, 64, 1, 4, 64, 64) == 0

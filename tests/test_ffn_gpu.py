@@ -257,6 +257,28 @@ def test_outputs_touch_nothing_else(m, n, pad, off):
         assert bool((buf == 123.0).all())
 
 
+@pytest.mark.parametrize("off", [(True, True), (True, False), (False, True)], ids=["both", "a", "b"])
+def test_rows_off_whole_sectors(off):
+    # Rows at odd multiples of 16 bytes (copied where that pays) hold what rows of whole sectors hold.
+    gen = torch.Generator().manual_seed(6)
+    m, n, k = 512, 8200, 4104
+    a, b, b2 = make(gen, BF16, m, k), weight(gen, BF16, k, n, "nk"), weight(gen, BF16, k, n, "nk")
+    dy = make(gen, BF16, m, n)
+
+    def padded(x, on):
+        return torch.nn.functional.pad(x, (0, 8))[:, :k] if on else x
+
+    def all_of(a, b, b2):
+        h, g, u = ffn.gated_linear(a, b, b2, return_preact=True)
+        return [ffn.fused_linear(a, b, activation="silu"), h, g, u,
+                *ffn.gated_linear_backward(dy, a, b, b2, g, u, has_bias=True)]
+
+    want = all_of(padded(a, True), padded(b.t(), True).t(), padded(b2.t(), True).t())
+    got = all_of(padded(a, not off[0]), padded(b.t(), not off[1]).t(), padded(b2.t(), not off[1]).t())
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    torch.testing.assert_close(want[0], torch.nn.functional.silu(a @ b), rtol=2.0 ** -6, atol=2.0 ** -6)
+
+
 def test_broadcast_residual_and_gradient():
     gen = torch.Generator().manual_seed(2)
     a, b = make(gen, BF16, 70, 64), weight(gen, BF16, 64, 96, "nk")
