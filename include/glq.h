@@ -354,7 +354,8 @@ enum glq_activation {
  *     value.
  *   - B with unit k stride (a weight W[N, K] as W^T) and with unit n stride
  *     are read as they lie, at 16-byte aligned bases and row pitches.  Other
- *     operands are first copied into the workspace.
+ *     operands are first copied into the workspace, and so are, in large
+ *     forward products where it pays, operands off 32 bytes.
  *   - workspace: device memory of at least the matching *_workspace_bytes()
  *     bytes, 256-byte aligned (GLQ_ERR_WORKSPACE otherwise; NULL when that is
  *     0; the size is that of the current device).  It holds nothing between
