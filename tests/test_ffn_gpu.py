@@ -276,6 +276,7 @@ def test_rows_off_whole_sectors(off):
     want = all_of(padded(a, True), padded(b.t(), True).t(), padded(b2.t(), True).t())
     got = all_of(padded(a, not off[0]), padded(b.t(), not off[1]).t(), padded(b2.t(), not off[1]).t())
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+    # Two roundings of y and one of z (slope of SiLU at most 1.1): 2^-8 each, of values that 2^-6 covers.
     torch.testing.assert_close(want[0], torch.nn.functional.silu(a @ b), rtol=2.0 ** -6, atol=2.0 ** -6)
 
 
