@@ -93,9 +93,11 @@ __device__ __forceinline__ void act_grad_f(float x, float* value, float* slope) 
     *value = x * cdf;
     *slope = fmaf(x * kInvSqrt2Pi, e, cdf);
   } else if constexpr (ACT == GLQ_ACT_GELU_TANH) {
-    const float s = sigmoid_f(kGeluC * x * (1.0f + kGeluCubic * x * x));
+    // s (1 - s) is 0 long before x^2 overflows, and has to meet a finite factor.
+    const float sq = fminf(x * x, 1e30f);
+    const float s = sigmoid_f(kGeluC * x * (1.0f + kGeluCubic * sq));
     *value = x * s;
-    *slope = s + x * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluCubic * x * x);
+    *slope = s + x * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluCubic * sq);
   } else if constexpr (ACT == GLQ_ACT_RELU) {
     *value = x > 0.0f || x != x ? x : 0.0f;
     *slope = x > 0.0f ? 1.0f : 0.0f;
