@@ -44,24 +44,35 @@ struct Elem16<__nv_bfloat16> {
 // sigmoid(x); exp(-x) overflows to infinity below -88, where the quotient is 0.
 __device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
-constexpr float kInvSqrt2 = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;  // density of the standard normal at 0
 constexpr float kGeluC = 1.59576912160573071f;       // 2 sqrt(2 / pi): tanh(t) = 2 sigmoid(2 t) - 1
 constexpr float kGeluCubic = 0.044715f;
 
-// Phi(x) of the exact GELU from e = exp(-x^2 / 2), which its derivative needs
-// anyway: erfc by formula 7.1.26 of Abramowitz and Stegun's Handbook of
-// Mathematical Functions (absolute error below 1.5e-7, i.e. 7.5e-8 here; the
-// 16-bit result's half-step is 2.4e-4 of it or more).  erff costs twice the
-// instructions and bounded the backward kernel (4096 x 11008: 80 us).
-__device__ __forceinline__ float normal_cdf(float x, float e) {
-  const float t = __fdividef(1.0f, fmaf(0.3275911f * kInvSqrt2, fabsf(x), 1.0f));
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  const float tail = 0.5f * p * t * e;
-  return x > 0.0f ? 1.0f - tail : tail;
+// exp(-x^2 / 2).
+__device__ __forceinline__ float gauss(float x) {
+  float e;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(x * x * -0.72134752044448170f));  // -1 / (2 ln 2)
+  return e;
+}
+
+// Phi(-|x|) of the exact GELU from e = gauss(x), which its derivative needs
+// anyway.  For negative x gelu(x) is x times this tail, so the error has to be
+// small against the tail itself: Phi(-|x|) / e falls smoothly from 1/2 like
+// 1 / |x|, and is t times a polynomial in t = 1 / (1 + 0.36 |x|), fitted here
+// (least squares of the relative error, reweighted towards its least maximum,
+// |x| up to 15): within 1.4e-6 of it with 32-bit evaluation.  e adds the
+// roundings of its argument, 2^-23 x^2 at most; the half-step of a 16-bit
+// result is 4.9e-4 or more.  erff costs twice the instructions and bounded the
+// backward kernel (4096 x 11008: 80 us), and 1 + erff cancels in the tail.
+__device__ __forceinline__ float normal_tail(float x, float e) {
+  const float t = __fdividef(1.0f, fmaf(0.36f, fabsf(x), 1.0f));
+  float p = fmaf(0.0465226406f, t, -0.17793574f);
+  p = fmaf(p, t, 0.178466204f);
+  p = fmaf(p, t, 0.0282575622f);
+  p = fmaf(p, t, 0.13909894f);
+  p = fmaf(p, t, 0.14188469f);
+  p = fmaf(p, t, 0.143705188f);
+  return p * t * e;
 }
 
 // act(x).  ACT is a glq_activation; the callers switch on it once per tile.
@@ -70,7 +81,8 @@ __device__ __forceinline__ float act_f(float x) {
   if constexpr (ACT == GLQ_ACT_SILU) {
     return x * sigmoid_f(x);
   } else if constexpr (ACT == GLQ_ACT_GELU) {
-    return x * normal_cdf(x, __expf(-0.5f * x * x));
+    // x Phi(x) = max(x, 0) - |x| Phi(-|x|); the cap keeps infinity from its tail of 0.
+    return fmaf(-fabsf(fminf(x, 1e30f)), normal_tail(x, gauss(x)), fmaxf(x, 0.0f));
   } else if constexpr (ACT == GLQ_ACT_GELU_TANH) {
     return x * sigmoid_f(kGeluC * x * (1.0f + kGeluCubic * x * x));
   } else if constexpr (ACT == GLQ_ACT_RELU) {
@@ -88,8 +100,9 @@ __device__ __forceinline__ void act_grad_f(float x, float* value, float* slope) 
     *value = x * s;
     *slope = s * (1.0f + x * (1.0f - s));
   } else if constexpr (ACT == GLQ_ACT_GELU) {
-    const float e = __expf(-0.5f * x * x);
-    const float cdf = normal_cdf(x, e);
+    const float e = gauss(x);
+    const float tail = normal_tail(x, e);
+    const float cdf = x > 0.0f ? 1.0f - tail : tail;
     *value = x * cdf;
     *slope = fmaf(x * kInvSqrt2Pi, e, cdf);
   } else if constexpr (ACT == GLQ_ACT_GELU_TANH) {

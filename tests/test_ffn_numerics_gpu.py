@@ -52,3 +52,59 @@ def test_slopes_of_huge_inputs(name):
     one = torch.ones_like(z)[None]
     dbias = ffn.gated_linear_backward(one, a, b, b, z[None], one, name, has_bias=True, need_a=False, need_b=False)[3]
     ref.within(dbias, want, bound, name)
+
+
+# Relative error of the 32-bit exact GELU's tail: its polynomial (2^-19 with its evaluation), the reciprocal and three
+# products (2^-21 together), and the exponential of -z^2/2, documented as 2 + 1.173 z^2 / 2 units of 2^-23, with the
+# rounding of z^2: below 2^-18 + 2^-23 z^2; twice the second term is allowed.
+def tail_error(z):
+    return 2.0 ** -18 + 2.0 ** -22 * z * z
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_exact_gelu_tail(m, dtype):
+    """Negative inputs, where the value is far smaller than its argument: bounds relative to the value.  The products
+    are exact (one term each), so the argument is the 16-bit z itself."""
+    z = torch.linspace(-13, -0.5, 2048, dtype=torch.float64).to(dtype).cuda()
+    a, w = torch.zeros((m, 8), dtype=dtype, device="cuda"), torch.zeros((z.numel(), 8), dtype=dtype, device="cuda")
+    a[:, 0] = 1.0
+    w[:, 0] = z
+    ones = torch.zeros_like(w)
+    ones[:, 0] = 1.0
+    zz = z.double()
+    want = ref.act(zz, "gelu")[0]
+    bound = (ref.unit(dtype) + tail_error(zz) * (1 + ref.unit(dtype))) * want.abs() + ref.tiny(dtype)
+    for y in (ffn.fused_linear(a, w.t(), activation="gelu"), ffn.gated_linear(a, w.t(), ones.t(), activation="gelu")):
+        ref.within(y, want.expand(m, -1), bound.expand(m, -1), "gelu")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_exact_gelu_slope_tail(dtype):
+    z = torch.linspace(-13, -0.5, 2048, dtype=torch.float64).to(dtype).cuda()
+    zz = z.double()
+    parts = 0.5 * torch.erfc(-zz / math.sqrt(2)) + zz.abs() * torch.exp(-zz * zz / 2) / math.sqrt(2 * math.pi)
+    want = ref.act(zz, "gelu")[1]
+    bound = ref.unit(dtype) * want.abs() + tail_error(zz) * (1 + ref.unit(dtype)) * parts + ref.tiny(dtype)
+    ref.within(slope_of(z, "gelu"), want, bound, "slope")
+    # In the gated backward pass, the value goes into the up projection's gradient.
+    a, b = torch.ones((1, 8), dtype=dtype, device="cuda"), torch.ones((z.numel(), 8), dtype=dtype, device="cuda").t()
+    one = torch.ones_like(z)[None]
+    dup = ffn.gated_linear_backward(one, a, b, b, z[None], one, "gelu", has_bias=True, need_a=False, need_b=False)[4]
+    value = ref.act(zz, "gelu")[0]
+    ref.within(dup, value, (ref.unit(dtype) + tail_error(zz) * (1 + ref.unit(dtype))) * value.abs() + ref.tiny(dtype),
+               "value")
+
+
+@pytest.mark.parametrize("name", [a for a in ref.ACTIVATIONS if a])
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_activations_of_the_largest_values(m, name):
+    """Infinity, the largest finite values and NaN (exact products of one term)."""
+    big = float(torch.finfo(BF16).max)
+    z = torch.tensor([math.inf, big, 2.0 ** 100, -big, -(2.0 ** 100), math.nan], dtype=BF16, device="cuda")
+    a, w = torch.zeros((m, 8), dtype=BF16, device="cuda"), torch.zeros((z.numel(), 8), dtype=BF16, device="cuda")
+    a[:, 0] = 1.0
+    w[:, 0] = z
+    y = ffn.fused_linear(a, w.t(), activation=name)
+    assert torch.equal(y[:, :3], z[:3].expand(m, 3)) and float(y[:, 3:5].abs().max()) == 0.0
+    assert bool(torch.isnan(y[:, 5]).all())
