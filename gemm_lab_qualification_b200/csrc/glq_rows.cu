@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
   __syncthreads();
   for (; r < a.rows; r += step) {
     const float rstd = next_rstd;
-    const float shift = -next_mean * rstd;  // xhat = x rstd + shift
+    const float mean = next_mean;
     if (r + step < a.rows) {
       next_mean = a.mean[r + step];
       next_rstd = a.rstd[r + step];
@@ -569,7 +569,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
         }
       }
     };
-    const Two rstd2 = two(rstd, rstd), shift2 = two(shift, shift);
+    // (x - mean is formed first: x rstd - mean rstd cancels in rows far off centre)
+    const Two rstd2 = two(rstd, rstd), minus_mean = two(-mean, -mean);
     Two s0 = 0, s1 = 0;  // sums of dy w xhat and of dy w
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -579,7 +580,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
       weights(j, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const Two t = mul2(g[i], fma2(xv[i], rstd2, shift2));
+        const Two t = mul2(g[i], mul2(add2(xv[i], minus_mean), rstd2));
         dw[j][i] = add2(dw[j][i], t);
         db[j][i] = add2(db[j][i], g[i]);
         s0 = fma2(t, w[i], s0);
@@ -591,10 +592,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
     // Past this join the whole group is done with the row before this one:
     // its slot takes the row kStages - 1 ahead.
     if (VEC && leads && ring.use > 1 && r + (kStages - 1) * step < a.rows) start(r + (kStages - 1) * step);
-    // dx = (rstd w) dy - rstd mean(g xhat) xhat - rstd mean(g)
+    // dx = (rstd w) dy - rstd^2 mean(g xhat) (x - mean) - rstd mean(g)
     const float k1 = -rstd * (sum[0] * inv), k2 = -rstd * (sum[1] * inv);
-    const float level1 = fmaf(shift, k1, k2);
-    const Two slope = two(k1 * rstd, k1 * rstd), level = two(level1, level1);
+    const Two slope = two(k1 * rstd, k1 * rstd), level = two(k2, k2);
     T* dx = static_cast<T*>(a.dx) + r * a.ld_dx;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) norm_backward_kernel(const Nor
       at(j, xv, g);
       weights(j, w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] = fma2(g[i], mul2(w[i], rstd2), fma2(xv[i], slope, level));
+      for (int i = 0; i < 4; ++i) g[i] = fma2(g[i], mul2(w[i], rstd2), fma2(add2(xv[i], minus_mean), slope, level));
       const uint4 raw = pack<T>(g);
       if constexpr (VEC) {
         *reinterpret_cast<uint4*>(dx + mine.column(j, 0)) = raw;

@@ -108,3 +108,24 @@ def test_activations_of_the_largest_values(m, name):
     y = ffn.fused_linear(a, w.t(), activation=name)
     assert torch.equal(y[:, :3], z[:3].expand(m, 3)) and float(y[:, 3:5].abs().max()) == 0.0
     assert bool(torch.isnan(y[:, 5]).all())
+
+
+@pytest.mark.parametrize("m,n", [(5, 256), (9, 1000), (40, 1001), (300, 4096), (40, 4095), (6, 8200), (4, 16384),
+                                 (3, 16392), (2, 20001)])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_layer_norm_backward_far_off_centre(m, n, dtype):
+    """Rows whose mean is hundreds of deviations (constant rows: any number) away from zero.  x - mean has one
+    rounding, so the bound is the one of the centred row."""
+    gen = torch.Generator().manual_seed(m + n)
+    step = 1000 * torch.finfo(dtype).eps
+    x = (1000 + torch.randint(-2, 3, (m, n), generator=gen) * step).to(dtype)
+    x[0] = 1000.0
+    x = x.cuda()
+    w, dy = make(gen, dtype, n, scale=0.2) + 1, make(gen, dtype, m, n)
+    mean = x.double().mean(1)
+    rstd = (x.double().var(1, unbiased=False) + 1e-5).rsqrt()
+    mean, rstd = mean.float(), rstd.float()
+    got = ffn.layer_norm_backward(dy, x, mean, rstd, w, has_bias=True)
+    want = ref.layer_norm_backward(d(dy), d(x) - d(mean)[:, None], torch.zeros_like(d(mean)), d(rstd), d(w), dtype)
+    for g, (v, bound), what in zip(got, want, ("dx", "dw", "db")):
+        ref.within(g, v, bound, what)
