@@ -355,7 +355,8 @@ __global__ void __launch_bounds__(G < kNormThreads ? kNormThreads : G, G < 512 ?
     if (r + step < a.rows) request(r + step);
     float sum[1] = {halves(acc).x + halves(acc).y};
     row_sum<G>(sum, my_red, phase, group);
-    const float mean = sum[0] * inv;
+    // (a division: the rounding of 1 / cols, times rstd, shows in constant rows)
+    const float mean = sum[0] / static_cast<float>(cols);
     const Two minus_mean = two(-mean, -mean);
     acc = 0;
 #pragma unroll
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a) {
       for (int i = 0; i < 8; ++i) sum[0] += v[i];
     }
     row_sum<1024>(sum, red, phase, 0);
-    const float mean = sum[0] * inv;
+    const float mean = sum[0] / static_cast<float>(a.cols);
     for (int c = threadIdx.x * 8; c < a.cols; c += 1024 * 8) {
       load8(x + c, a.align, a.cols - c, v);
       for (int i = 0; i < 8; ++i) {

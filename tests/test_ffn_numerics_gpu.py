@@ -129,3 +129,16 @@ def test_layer_norm_backward_far_off_centre(m, n, dtype):
     want = ref.layer_norm_backward(d(dy), d(x) - d(mean)[:, None], torch.zeros_like(d(mean)), d(rstd), d(w), dtype)
     for g, (v, bound), what in zip(got, want, ("dx", "dw", "db")):
         ref.within(g, v, bound, what)
+
+
+@pytest.mark.parametrize("n", [100, 251, 513, 1001, 2047, 4095, 8190, 12001, 20001])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_layer_norm_of_constant_rows(n, dtype):
+    """Every partial sum of rows of 1000 or 7 is exact, and so is their quotient by n: deviations are exactly zero
+    (one last bit of the mean would come out as 1000 * 2^-24 * 316, far above the bias)."""
+    x = torch.tensor([[1000.0], [7.0], [-1000.0]], dtype=dtype, device="cuda").expand(3, n).contiguous()
+    bias = torch.linspace(-1, 1, n).to(dtype).cuda()
+    y, mean, rstd = ffn.layer_norm(x, None, bias, 1e-5, return_stats=True)
+    assert torch.equal(mean, x[:, 0].float())
+    assert torch.equal(y, bias.expand(3, n))
+    assert float((rstd.double() * math.sqrt(1e-5) - 1).abs().max()) <= 2.0 ** -21
