@@ -644,8 +644,8 @@ int glq_layer_norm(int dtype, const void* X, int64_t x_row_stride, const void* w
   if (v != GLQ_OK) return v;
   if (M < 0 || M > INT_MAX) return GLQ_ERR_SHAPE;
   if (!(eps >= 0.0) || (mean == nullptr) != (rstd == nullptr)) return GLQ_ERR_INVALID_ARGUMENT;
-  if (M == 0 || N == 0) return GLQ_OK;
-  if (X == nullptr || Y == nullptr) return GLQ_ERR_INVALID_ARGUMENT;
+  if (M == 0 || (N == 0 && mean == nullptr)) return GLQ_OK;
+  if (N > 0 && (X == nullptr || Y == nullptr)) return GLQ_ERR_INVALID_ARGUMENT;
   if (glq::odd(X) || glq::odd(Y) || glq::odd(weight) || glq::odd(bias) || !glq::aligned(mean, 4) ||
       !glq::aligned(rstd, 4)) {
     return GLQ_ERR_INVALID_ARGUMENT;
@@ -656,6 +656,13 @@ int glq_layer_norm(int dtype, const void* X, int64_t x_row_stride, const void* w
   unsigned int* err = nullptr;
   const int d = glq::current_device(&sm_count, &err);
   if (d != GLQ_OK) return d;
+  if (N == 0) {
+    // Statistics of no values, 0 / 0: all bits set are a NaN.
+    const size_t bytes = static_cast<size_t>(M) * sizeof(float);
+    cudaError_t e = cudaMemsetAsync(mean, 0xff, bytes, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) e = cudaMemsetAsync(rstd, 0xff, bytes, static_cast<cudaStream_t>(stream));
+    return glq::status_of(e);
+  }
   glq::NormArgs a = {};
   a.x = X;
   a.ld_x = x_row_stride;

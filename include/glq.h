@@ -458,7 +458,7 @@ size_t glq_gated_linear_backward_workspace_bytes(int dtype, const void* A, int64
  * glq_layer_norm -- Y[m, :] = (X[m, :] - mean_m) * rstd_m * weight + bias with
  * mean_m the row's mean and rstd_m = 1 / sqrt(mean((X[m, :] - mean_m)^2) + eps).
  * weight and bias [N] are optional; mean and rstd (FP32 [M], both or neither)
- * are what the backward pass reads.
+ * are what the backward pass reads; for rows without elements they are NaN.
  */
 int glq_layer_norm(int dtype, const void* X, int64_t x_row_stride, const void* weight, const void* bias, double eps,
                    void* Y, int64_t y_row_stride, float* mean, float* rstd, int64_t M, int64_t N,

@@ -142,3 +142,11 @@ def test_layer_norm_of_constant_rows(n, dtype):
     assert torch.equal(mean, x[:, 0].float())
     assert torch.equal(y, bias.expand(3, n))
     assert float((rstd.double() * math.sqrt(1e-5) - 1).abs().max()) <= 2.0 ** -21
+
+
+def test_statistics_of_empty_rows():
+    """The mean of no values is 0 / 0, and so is their variance: not what the memory held before."""
+    torch.full((3,), 7.0, device="cuda")  # the block that the statistics will take
+    torch.full((3,), 7.0, device="cuda")
+    y, mean, rstd = ffn.layer_norm(torch.empty((3, 0), dtype=F16, device="cuda"), return_stats=True)
+    assert y.shape == (3, 0) and bool(torch.isnan(mean).all()) and bool(torch.isnan(rstd).all())
