@@ -63,6 +63,12 @@ void check_bias(const at::Tensor& bias, const at::Tensor& a, int64_t n) {
   if (n > 1 && bias.stride(0) != 1) throw py::value_error("bias tensor must be contiguous");
 }
 
+// What the kernels write through a raw pointer: autograd compares the version
+// of a tensor it saved with the present one (inference tensors have none).
+void wrote(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Returns (glq_status, path, split).  `op` names the operator in messages.
 std::tuple<int, int, int> linear(const std::string& op, const at::Tensor& a, const at::Tensor& b, at::Tensor& out,
                                  const c10::optional<at::Tensor>& bias, int epilogue, int split_k,
@@ -97,6 +103,7 @@ std::tuple<int, int, int> linear(const std::string& op, const at::Tensor& a, con
                                    bias.has_value() ? bias->data_ptr() : nullptr, epilogue, out.data_ptr(),
                                    out.stride(0), m, n, k, split_k, ws, ws_bytes, stream,
                                    static_cast<unsigned int>(flags), &path, &split);
+  wrote(out);
   return {status, path, split};
 }
 
@@ -213,6 +220,8 @@ std::tuple<int, at::Tensor, OptTensor> fused_linear(const at::Tensor& a, const a
       dtype_of(a), a.data_ptr(), a.stride(0), a.stride(1), b.data_ptr(), b.stride(0), b.stride(1), ptr(bias), activation,
       res.defined() ? res.data_ptr() : nullptr, res.defined() ? res.stride(0) : 0, ptr(z), z.has_value() ? z->stride(0) : 0,
       y.data_ptr(), y.stride(0), m, n, k, ws.data(), ws.bytes, stream_of(a), static_cast<unsigned int>(flags));
+  if (output.has_value()) wrote(y);
+  if (preact.has_value()) wrote(*z);
   return {status, y, z};
 }
 
@@ -289,6 +298,11 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> gated_linear(const at::Tensor&
       b_up.data_ptr(), b_up.stride(0), b_up.stride(1), ptr(bias_gate), ptr(bias_up), activation,
       ptr(g), ptr(u), g.has_value() ? g->stride(0) : 0, y.data_ptr(), y.stride(0),
       m, n, k, ws.data(), ws.bytes, stream_of(a), static_cast<unsigned int>(flags));
+  if (output.has_value()) wrote(y);
+  if (gate.has_value()) {
+    wrote(*g);
+    wrote(*u);
+  }
   return {status, y, g, u};
 }
 
@@ -363,6 +377,7 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm(const at::Tensor& x
                                     y.data_ptr(), y.stride(0), return_stats ? mean->data_ptr<float>() : nullptr,
                                     return_stats ? rstd->data_ptr<float>() : nullptr, m, n, stream_of(x),
                                     static_cast<unsigned int>(flags));
+  if (output.has_value()) wrote(y);
   return {status, y, mean, rstd};
 }
 

@@ -23,6 +23,10 @@ the inputs' 16-bit type; every sum is FP32 with one rounding, except that the
 gradient of the pre-activations is rounded to 16 bits before the products that
 read it.  The backward passes themselves are not differentiable.
 
+The ``*_into`` forms write in place and raise the version of what they wrote,
+as torch's own operations do: a pending backward pass that saved the tensor
+then ends with torch's error instead of with wrong gradients.
+
 Results are the same bits on every run of the same call; which gradients are
 asked for together may change the order of their sums.  All calls can be
 captured into CUDA graphs after a first call on the device.  To capture a

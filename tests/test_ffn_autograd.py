@@ -1,0 +1,57 @@
+"""What torch has to know about the feed-forward operators: tensors written in place, forward-mode tangents, what a
+call keeps and computes for its backward pass, and ahead-of-time tracing."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from gemm_lab_qualification_b200 import ffn, kernels
+
+F16 = torch.float16
+
+
+# ---------------------------------------------------------------- tensors written in place
+
+def matrices(n, size=64):
+    gen = torch.Generator().manual_seed(n)
+    return [torch.randn(size, size, generator=gen).to(F16).cuda() for _ in range(n)]
+
+
+def writers():
+    """(name, call that writes its first argument from the others)"""
+    return [
+        ("fused_linear_into", lambda out, a, b, c: ffn.fused_linear_into(a, b, out, residual=out)),
+        ("preact", lambda out, a, b, c: ffn.fused_linear_into(a, b, c, activation="silu", preact=out)),
+        ("gated_linear_into", lambda out, a, b, c: ffn.gated_linear_into(a, b, b, out)),
+        ("gate", lambda out, a, b, c: ffn.gated_linear_into(a, b, b, c, gate=out, up=torch.empty_like(c))),
+        ("up", lambda out, a, b, c: ffn.gated_linear_into(a, b, b, c, gate=torch.empty_like(c), up=out)),
+        ("layer_norm_into", lambda out, a, b, c: ffn.layer_norm_into(a, out)),
+        ("triton_matmul_into", lambda out, a, b, c: kernels.triton_matmul_into(a, b, out)),
+        ("triton_bias_silu_into", lambda out, a, b, c: kernels.triton_bias_silu_into(a, b, a[0], out)),
+    ]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,write", writers(), ids=[w[0] for w in writers()])
+def test_writes_raise_the_version(cuda_device, name, write):
+    """A tensor that a pending backward pass has saved cannot be overwritten unseen."""
+    x, a, b, c = matrices(4)
+    weight = torch.ones(64, dtype=F16, device="cuda", requires_grad=True)
+    y = ffn.layer_norm(x, weight)  # saves x
+    before = x._version
+    write(x, a, b, c)
+    assert x._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_inputs_and_inference_tensors_keep_their_version(cuda_device):
+    x, a, b, c = matrices(4)
+    for _, write in writers():
+        write(x, a, b, c)
+    assert a._version == 0 and b._version == 0
+    with torch.inference_mode():
+        frozen = torch.empty_like(x)
+    for _, write in writers():
+        write(frozen, a, b, c)  # (has no version to raise)
