@@ -166,6 +166,15 @@ void check_matrix(const at::Tensor& t, const at::Tensor& a, int64_t m, int64_t n
   }
 }
 
+// A caller's output.  One that autograd follows would keep the history, and so
+// the gradients, of the values that the call overwrites.
+void check_written(const at::Tensor& out, const at::Tensor& a, int64_t m, int64_t n) {
+  check_output(out, a, m, n);
+  if (at::GradMode::is_enabled() && out.requires_grad()) {
+    throw py::value_error("an output tensor requires gradients; write it under torch.no_grad()");
+  }
+}
+
 // An input read by rows: itself if its columns are contiguous and its rows
 // do not overlap, else a contiguous copy.
 at::Tensor by_rows(const at::Tensor& t) {
@@ -206,10 +215,10 @@ std::tuple<int, at::Tensor, OptTensor> fused_linear(const at::Tensor& a, const a
     res = by_rows(*residual);
   }
   at::Tensor y = output.has_value() ? *output : at::empty({m, n}, a.options());
-  if (output.has_value()) check_output(y, a, m, n);
+  if (output.has_value()) check_written(y, a, m, n);
   OptTensor z = preact;
   if (z.has_value()) {
-    check_output(*z, a, m, n);
+    check_written(*z, a, m, n);
   } else if (return_preact) {
     z = at::empty({m, n}, a.options());
   }
@@ -276,12 +285,12 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> gated_linear(const at::Tensor&
   check_vector(bias_gate, a, n, "bias_gate");
   check_vector(bias_up, a, n, "bias_up");
   at::Tensor y = output.has_value() ? *output : at::empty({m, n}, a.options());
-  if (output.has_value()) check_output(y, a, m, n);
+  if (output.has_value()) check_written(y, a, m, n);
   OptTensor g = gate, u = up;
   if (g.has_value() != u.has_value()) throw py::value_error("gate and up are given together");
   if (g.has_value()) {
-    check_output(*g, a, m, n);
-    check_output(*u, a, m, n);
+    check_written(*g, a, m, n);
+    check_written(*u, a, m, n);
     if (m > 1 && g->stride(0) != u->stride(0)) throw py::value_error("gate and up need one row stride");
   } else if (return_preact) {
     g = at::empty({m, n}, a.options());
@@ -367,7 +376,7 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm(const at::Tensor& x
   check_vector(bias, x, n, "bias");
   const at::Tensor rows = by_rows(x);
   at::Tensor y = output.has_value() ? *output : at::empty({m, n}, x.options());
-  if (output.has_value()) check_output(y, x, m, n);
+  if (output.has_value()) check_written(y, x, m, n);
   OptTensor mean, rstd;
   if (return_stats) {
     mean = at::empty({m}, x.options().dtype(at::kFloat));

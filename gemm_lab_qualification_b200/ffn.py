@@ -25,7 +25,9 @@ read it.  The backward passes themselves are not differentiable.
 
 The ``*_into`` forms write in place and raise the version of what they wrote,
 as torch's own operations do: a pending backward pass that saved the tensor
-then ends with torch's error instead of with wrong gradients.
+then ends with torch's error instead of with wrong gradients.  They are not
+differentiable, and while gradients are recorded they refuse an output that
+requires them.
 
 Results are the same bits on every run of the same call; which gradients are
 asked for together may change the order of their sums.  All calls can be

@@ -55,3 +55,21 @@ def test_inputs_and_inference_tensors_keep_their_version(cuda_device):
         frozen = torch.empty_like(x)
     for _, write in writers():
         write(frozen, a, b, c)  # (has no version to raise)
+
+
+@pytest.mark.gpu
+def test_outputs_that_autograd_follows_are_refused(cuda_device):
+    """Writing a tensor that requires gradients would leave it the history, and the gradients, of what it held."""
+    x, a, b, c = matrices(4)
+    for out in (x.clone().requires_grad_(), x.clone().requires_grad_() * 1):
+        was = out.detach().clone()
+        for name, write in writers()[:6]:
+            with pytest.raises(ValueError, match="requires gradients"):
+                write(out, a, b, c)
+        assert torch.equal(out.detach(), was)
+    # An optimizer's or a decoder's writes are outside autograd.
+    with torch.no_grad():
+        for name, write in writers():
+            write(out, a, b, c)
+    # Inputs may require gradients: the call is documented as not differentiable.
+    assert not ffn.fused_linear_into(a.requires_grad_(), b, c).requires_grad
