@@ -9,8 +9,10 @@
 // contiguity rule) and the launch in one native call on torch's current
 // stream.  Library failures come back as the glq_status so that Python raises
 // the same GlqError as the ctypes binding.
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/extension.h>
 
 #include <sstream>
@@ -151,6 +153,20 @@ cudaStream_t stream_of(const at::Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
 
+// The operators have no forward-mode derivative: an output without a tangent
+// would stand for a derivative of zero.
+bool dual(const at::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool dual(const OptTensor& t) { return t.has_value() && dual(*t); }
+
+template <typename... Tensors>
+void check_no_tangent(const char* op, const Tensors&... tensors) {
+  // (outside of every dual level there are none; asking each tensor costs views 0.1 us)
+  if (torch::autograd::ForwardADLevel::try_get_by_idx(0) == nullptr) return;
+  if ((dual(tensors) || ...) && c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+    throw py::value_error(std::string(op) + " has no forward-mode derivative");
+  }
+}
+
 void check_vector(const OptTensor& v, const at::Tensor& a, int64_t n, const char* name) {
   if (!v.has_value()) return;
   if (v->dim() != 1 || v->size(0) != n || v->device() != a.device() || v->scalar_type() != a.scalar_type()) {
@@ -205,6 +221,7 @@ at::Tensor empty_like_weight(const at::Tensor& b) {
 std::tuple<int, at::Tensor, OptTensor> fused_linear(const at::Tensor& a, const at::Tensor& b, const OptTensor& bias,
                                                     int activation, const OptTensor& residual, const OptTensor& output,
                                                     const OptTensor& preact, bool return_preact, int64_t flags) {
+  check_no_tangent("fused_linear", a, b, bias, residual, output, preact);
   check_inputs(a, b, "fused_linear");
   const c10::cuda::CUDAGuard guard(a.device());
   const int64_t m = a.size(0), k = a.size(1), n = b.size(1);
@@ -238,6 +255,7 @@ std::tuple<int, OptTensor, OptTensor, OptTensor> fused_linear_backward(const at:
                                                                        const at::Tensor& b, const OptTensor& preact,
                                                                        int activation, bool want_a, bool want_b,
                                                                        bool has_bias, int64_t flags) {
+  check_no_tangent("fused_linear_backward", grad, a, b, preact);
   check_inputs(a, b, "fused_linear_backward");
   const c10::cuda::CUDAGuard guard(a.device());
   const int64_t m = a.size(0), k = a.size(1), n = b.size(1);
@@ -279,6 +297,7 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> gated_linear(const at::Tensor&
                                                                const OptTensor& bias_up, int activation,
                                                                const OptTensor& output, const OptTensor& gate,
                                                                const OptTensor& up, bool return_preact, int64_t flags) {
+  check_no_tangent("gated_linear", a, b_gate, b_up, bias_gate, bias_up, output, gate, up);
   check_pair(a, b_gate, b_up, "gated_linear");
   const c10::cuda::CUDAGuard guard(a.device());
   const int64_t m = a.size(0), k = a.size(1), n = b_gate.size(1);
@@ -319,6 +338,7 @@ std::tuple<int, OptTensor, OptTensor, OptTensor, OptTensor, OptTensor> gated_lin
     const at::Tensor& grad, const at::Tensor& a, const at::Tensor& b_gate, const at::Tensor& b_up,
     const at::Tensor& gate, const at::Tensor& up, int activation, bool want_a, bool want_b, bool has_bias,
     int64_t flags) {
+  check_no_tangent("gated_linear_backward", grad, a, b_gate, b_up, gate, up);
   check_pair(a, b_gate, b_up, "gated_linear_backward");
   const c10::cuda::CUDAGuard guard(a.device());
   const int64_t m = a.size(0), k = a.size(1), n = b_gate.size(1);
@@ -369,6 +389,7 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm(const at::Tensor& x
                                                              const OptTensor& bias, double eps,
                                                              const OptTensor& output, bool return_stats,
                                                              int64_t flags) {
+  check_no_tangent("layer_norm", x, weight, bias, output);
   check_norm(x, "layer_norm");
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t m = x.size(0), n = x.size(1);
@@ -394,6 +415,7 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm_backward(const at::
                                                                       const at::Tensor& mean, const at::Tensor& rstd,
                                                                       const OptTensor& weight, bool has_bias,
                                                                       int64_t flags) {
+  check_no_tangent("layer_norm_backward", grad, x, mean, rstd, weight);
   check_norm(x, "layer_norm_backward");
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t m = x.size(0), n = x.size(1);

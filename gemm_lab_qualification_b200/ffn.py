@@ -21,7 +21,8 @@ tracing), which keeps what its backward pass reads.  The ``*_backward``
 functions are those passes for callers that run their own.  Gradients have
 the inputs' 16-bit type; every sum is FP32 with one rounding, except that the
 gradient of the pre-activations is rounded to 16 bits before the products that
-read it.  The backward passes themselves are not differentiable.
+read it.  The backward passes themselves are not differentiable,
+and forward-mode tangents (``torch.autograd.forward_ad``) are refused.
 
 The ``*_into`` forms write in place and raise the version of what they wrote,
 as torch's own operations do: a pending backward pass that saved the tensor

@@ -4,10 +4,47 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from gemm_lab_qualification_b200 import ffn, kernels
 
 F16 = torch.float16
+
+
+# ---------------------------------------------------------------- forward mode
+
+def dual(*shape):
+    t = torch.zeros(*shape, dtype=F16)
+    return fwd.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.parametrize("call", [
+    lambda x, p: ffn.fused_linear(x, p), lambda x, p: ffn.fused_linear(p, x.t()),
+    lambda x, p: ffn.fused_linear(p, p, x[0]), lambda x, p: ffn.fused_linear(p, p, None, None, x),
+    lambda x, p: ffn.fused_linear_into(x, p, torch.zeros_like(p)), lambda x, p: ffn.fused_linear_into(p, p, x),
+    lambda x, p: ffn.fused_linear_backward(x, p, p),
+    lambda x, p: ffn.gated_linear(p, p, x), lambda x, p: ffn.gated_linear_into(p, p, p, x),
+    lambda x, p: ffn.gated_linear_backward(p, p, p, p, x, p),
+    lambda x, p: ffn.layer_norm(x), lambda x, p: ffn.layer_norm(p, x[0]), lambda x, p: ffn.layer_norm_into(x, p),
+    lambda x, p: ffn.layer_norm_backward(x, p, p[0].float(), p[0].float()),
+    lambda x, p: ffn.feed_forward(x, p, p, p),
+])
+def test_forward_mode_tangents_are_refused(call):
+    """An output without a tangent would be a derivative of zero."""
+    with fwd.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        call(dual(8, 8), torch.zeros(8, 8, dtype=F16))
+
+
+@pytest.mark.gpu
+def test_forward_mode_of_trainable_tensors(cuda_device):
+    x, w = (torch.randn(8, 8, device="cuda").half() for _ in range(2))
+    with fwd.dual_level():
+        for t in (x, x.clone().requires_grad_()):
+            with pytest.raises(Exception):
+                ffn.fused_linear(fwd.make_dual(t, torch.ones_like(x)), w)
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda v: ffn.layer_norm(v), (x,), (torch.ones_like(x),))
+    assert ffn.fused_linear(x, w).shape == (8, 8)
 
 
 # ---------------------------------------------------------------- tensors written in place
