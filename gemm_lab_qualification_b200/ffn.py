@@ -99,15 +99,12 @@ def fused_linear_into(a: Tensor, b: Tensor, output: Tensor, bias: Tensor | None 
 def fused_linear(a: Tensor, b: Tensor, bias: Tensor | None = None, activation: str | None = None,
                  residual: Tensor | None = None, return_preact: bool = False):
     """act(a @ b + bias) + residual; with return_preact, also ``a @ b + bias``
-    (the backward pass reads it; None stays differentiable only through the
-    first output)."""
+    (what the backward pass of an activation reads; differentiable only
+    through the first output)."""
     if _differentiable(a, b, bias, residual):
-        y, z = fused_linear_op(a, b, bias, activation, residual)
-        if not return_preact:
-            return y
-        # Without an activation and a residual the output is the pre-activation.
-        return y, (z if activation is not None else _fused_linear(a.detach(), b.detach(), bias, None, None)[0])
-    y, z = _fused_linear(a, b, bias, activation, residual, return_preact=return_preact)
+        y, z = fused_linear_op(a, b, bias, activation, residual, return_preact)
+    else:
+        y, z = _fused_linear(a, b, bias, activation, residual, return_preact=return_preact)
     return (y, z) if return_preact else y
 
 
@@ -227,19 +224,20 @@ def _weight_order(b: Tensor) -> Tensor:
 
 @torch.library.custom_op("gemm_lab::fused_linear", mutates_args=())
 def fused_linear_op(a: Tensor, b: Tensor, bias: Optional[Tensor], activation: Optional[str],
-                    residual: Optional[Tensor]) -> tuple[Tensor, Tensor]:
-    """(act(a @ b + bias) + residual, a @ b + bias or empty without activation)."""
-    y, z = _fused_linear(a, b, bias, activation, residual, return_preact=activation is not None)
+                    residual: Optional[Tensor], keep_preact: bool = False) -> tuple[Tensor, Tensor]:
+    """(act(a @ b + bias) + residual, a @ b + bias); the latter is empty
+    without an activation unless keep_preact asks for it."""
+    y, z = _fused_linear(a, b, bias, activation, residual, return_preact=activation is not None or keep_preact)
     return y, _or_empty(z, a)
 
 
 @fused_linear_op.register_fake
-def _(a, b, bias, activation, residual):
+def _(a, b, bias, activation, residual, keep_preact=False):
     _activation(activation)
     if a.ndim != 2 or b.ndim != 2 or a.shape[1] != b.shape[0]:
         raise ValueError("incompatible matrix shapes")
     y = a.new_empty((a.shape[0], b.shape[1]))
-    return y, (torch.empty_like(y) if activation is not None else a.new_empty(0))
+    return y, (torch.empty_like(y) if activation is not None or keep_preact else a.new_empty(0))
 
 
 @torch.library.custom_op("gemm_lab::fused_linear_backward", mutates_args=())
@@ -257,8 +255,8 @@ def _(grad_output, a, b, preact, activation, has_bias, need_a, need_b):
 
 
 def _fused_linear_setup(ctx, inputs, output):
-    a, b, bias, activation, residual = inputs
-    ctx.save_for_backward(a, b, output[1])
+    a, b, bias, activation, residual, _ = inputs
+    ctx.save_for_backward(a, b, output[1] if activation is not None else None)
     ctx.activation, ctx.has_bias = activation, bias is not None
     ctx.mark_non_differentiable(output[1])
 
@@ -269,9 +267,10 @@ def _fused_linear_grad(ctx, grad_y, _):
     want_bias = ctx.has_bias and need[2]
     da = db = dbias = None
     if need[0] or need[1] or want_bias:
-        da, db, dbias = fused_linear_backward_op(grad_y, a, b, z, ctx.activation, want_bias, need[0], need[1])
+        da, db, dbias = fused_linear_backward_op(grad_y, a, b, _or_empty(z, a), ctx.activation, want_bias, need[0],
+                                                 need[1])
     return (da if need[0] else None, db if need[1] else None, dbias if want_bias else None, None,
-            grad_y if need[4] else None)
+            grad_y if need[4] else None, None)
 
 
 fused_linear_op.register_autograd(_fused_linear_grad, setup_context=_fused_linear_setup)

@@ -110,3 +110,67 @@ def test_outputs_that_autograd_follows_are_refused(cuda_device):
             write(out, a, b, c)
     # Inputs may require gradients: the call is documented as not differentiable.
     assert not ffn.fused_linear_into(a.requires_grad_(), b, c).requires_grad
+
+
+# ---------------------------------------------------------------- what a call runs
+
+class FakeBinding:
+    """Counts the native calls, and answers them on the CPU."""
+
+    def __init__(self):
+        self.calls = []
+
+    def fused_linear(self, a, b, bias, act, residual, output, preact, return_preact, flags):
+        self.calls.append("fused_linear")
+        z = a @ b if bias is None else a @ b + bias
+        y = z.clone() if residual is None else z + residual
+        return 0, y, z.clone() if return_preact else None
+
+    def fused_linear_backward(self, dy, a, b, z, act, want_a, want_b, has_bias, flags):
+        self.calls.append("fused_linear_backward")
+        return (0, dy @ b.t() if want_a else None, a.t() @ dy if want_b else None, dy.sum(0) if has_bias else None)
+
+    def layer_norm(self, x, weight, bias, eps, output, return_stats, flags):
+        return 0, x.clone(), x.float().mean(1), torch.ones(x.shape[0])
+
+    def layer_norm_backward(self, dy, x, mean, rstd, weight, has_bias, need_weight, flags):
+        self.calls.append(("layer_norm_backward", has_bias, need_weight))
+        return (0, dy.clone(), dy.sum(0) if weight is not None and need_weight else None,
+                dy.sum(0) if has_bias else None)
+
+
+@pytest.fixture
+def native_calls(monkeypatch):
+    fake = FakeBinding()
+    monkeypatch.setattr(ffn, "_binding", lambda: fake)
+    return fake.calls
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_kept_preactivation_costs_no_second_product(native_calls, residual):
+    """Without an activation the one product gives both results."""
+    gen = torch.Generator().manual_seed(1)
+    a, b, r = (torch.randn(4, 4, generator=gen, dtype=torch.float64).requires_grad_() for _ in range(3))
+    y, z = ffn.fused_linear(a, b, None, None, r if residual else None, return_preact=True)
+    assert native_calls == ["fused_linear"]
+    assert torch.equal(z, (a @ b).detach()) and not z.requires_grad
+    assert y.data_ptr() != z.data_ptr()
+    y.backward(torch.ones_like(y))
+    assert native_calls == ["fused_linear", "fused_linear_backward"]
+    assert torch.equal(a.grad, torch.ones_like(y) @ b.detach().t())
+    native_calls.clear()
+    assert ffn.fused_linear(a, b).requires_grad and native_calls == ["fused_linear"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40, 300])
+@pytest.mark.parametrize("activation", [None, "gelu"])
+def test_kept_preactivation_is_the_same_with_gradients(cuda_device, m, activation):
+    gen = torch.Generator().manual_seed(m)
+    a, w = torch.randn(m, 72, generator=gen).to(F16).cuda(), torch.randn(136, 72, generator=gen).to(F16).cuda()
+    r = torch.randn(m, 136, generator=gen).to(F16).cuda()
+    for res in (None, r):
+        want = ffn.fused_linear(a, w.t(), None, activation, res, return_preact=True)
+        got = ffn.fused_linear(a.clone().requires_grad_(), w.t(), None, activation, res, return_preact=True)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        assert got[0].requires_grad and not got[1].requires_grad
