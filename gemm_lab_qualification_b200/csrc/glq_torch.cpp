@@ -413,7 +413,7 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm(const at::Tensor& x
 
 std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm_backward(const at::Tensor& grad, const at::Tensor& x,
                                                                       const at::Tensor& mean, const at::Tensor& rstd,
-                                                                      const OptTensor& weight, bool has_bias,
+                                                                      const OptTensor& weight, bool has_bias, bool need_weight,
                                                                       int64_t flags) {
   check_no_tangent("layer_norm_backward", grad, x, mean, rstd, weight);
   check_norm(x, "layer_norm_backward");
@@ -430,9 +430,9 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm_backward(const at::
   const at::Tensor dy = by_rows(grad), rows = by_rows(x);
   at::Tensor dx = at::empty({m, n}, x.options());
   OptTensor dweight, dbias;
-  if (weight.has_value()) dweight = at::empty({n}, x.options());
+  if (weight.has_value() && need_weight) dweight = at::empty({n}, x.options());
   if (has_bias) dbias = at::empty({n}, x.options());
-  const Workspace ws(weight.has_value() || has_bias ? glq_layer_norm_backward_workspace_bytes(m, n) : 0, x);
+  const Workspace ws(dweight.has_value() || has_bias ? glq_layer_norm_backward_workspace_bytes(m, n) : 0, x);
   const int status = glq_layer_norm_backward(
       dtype_of(x), dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), ptr(weight), mean.data_ptr<float>(),
       rstd.data_ptr<float>(), dx.data_ptr(), dx.stride(0), ptr(dweight),

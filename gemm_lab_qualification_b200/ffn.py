@@ -190,9 +190,12 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
 
 
 def layer_norm_backward(grad_output: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, weight: Tensor | None = None,
-                        has_bias: bool = False) -> tuple[Tensor, Tensor | None, Tensor | None]:
-    """(grad x, grad weight, grad bias) of ``layer_norm``."""
-    status, dx, dweight, dbias = _binding().layer_norm_backward(grad_output, x, mean, rstd, weight, has_bias, _flags())
+                        has_bias: bool = False,
+                        need_weight: bool = True) -> tuple[Tensor, Tensor | None, Tensor | None]:
+    """(grad x, grad weight, grad bias) of ``layer_norm``; need_weight False
+    leaves out the gradient of a weight that is not trained."""
+    status, dx, dweight, dbias = _binding().layer_norm_backward(grad_output, x, mean, rstd, weight, has_bias,
+                                                                need_weight, _flags())
     _check(status, "glq_layer_norm_backward")
     return dx, dweight, dbias
 
@@ -342,14 +345,15 @@ def _(x, weight, bias, eps):
 
 @torch.library.custom_op("gemm_lab::layer_norm_backward", mutates_args=())
 def layer_norm_backward_op(grad_output: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, weight: Optional[Tensor],
-                           has_bias: bool) -> tuple[Tensor, Tensor, Tensor]:
-    return tuple(_or_empty(g, x) for g in layer_norm_backward(grad_output, x, mean, rstd, weight, has_bias))
+                           has_bias: bool, need_weight: bool = True) -> tuple[Tensor, Tensor, Tensor]:
+    return tuple(_or_empty(g, x) for g in layer_norm_backward(grad_output, x, mean, rstd, weight, has_bias, need_weight))
 
 
 @layer_norm_backward_op.register_fake
-def _(grad_output, x, mean, rstd, weight, has_bias):
+def _(grad_output, x, mean, rstd, weight, has_bias, need_weight=True):
     n = x.shape[1]
-    return (x.new_empty(x.shape), x.new_empty(n if weight is not None else 0), x.new_empty(n if has_bias else 0))
+    return (x.new_empty(x.shape), x.new_empty(n if weight is not None and need_weight else 0),
+            x.new_empty(n if has_bias else 0))
 
 
 def _layer_norm_setup(ctx, inputs, output):
@@ -361,7 +365,7 @@ def _layer_norm_setup(ctx, inputs, output):
 def _layer_norm_grad(ctx, grad_y, *_):
     x, weight, mean, rstd = ctx.saved_tensors
     need = ctx.needs_input_grad
-    dx, dweight, dbias = layer_norm_backward_op(grad_y, x, mean, rstd, weight, need[2])
+    dx, dweight, dbias = layer_norm_backward_op(grad_y, x, mean, rstd, weight, need[2], need[1])
     return dx if need[0] else None, dweight if need[1] else None, dbias if need[2] else None, None
 
 

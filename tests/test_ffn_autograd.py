@@ -174,3 +174,24 @@ def test_kept_preactivation_is_the_same_with_gradients(cuda_device, m, activatio
         got = ffn.fused_linear(a.clone().requires_grad_(), w.t(), None, activation, res, return_preact=True)
         assert all(torch.equal(x, y) for x, y in zip(got, want))
         assert got[0].requires_grad and not got[1].requires_grad
+
+
+@pytest.mark.parametrize("frozen", [True, False])
+def test_frozen_norm_weights_cost_no_gradient(native_calls, frozen):
+    x, weight = torch.randn(3, 4, requires_grad=True), torch.ones(4, requires_grad=not frozen)
+    ffn.layer_norm(x, weight).sum().backward()
+    assert native_calls == [("layer_norm_backward", False, not frozen)]
+    assert (weight.grad is None) == frozen and x.grad is not None
+
+
+@pytest.mark.gpu
+def test_layer_norm_backward_without_the_weights_gradient(cuda_device):
+    gen = torch.Generator().manual_seed(2)
+    x, dy = (torch.randn(40, 264, generator=gen).to(F16).cuda() for _ in range(2))
+    w = torch.randn(264, generator=gen).to(F16).cuda()
+    _, mean, rstd = ffn.layer_norm(x, w, return_stats=True)
+    dx, dw, db = ffn.layer_norm_backward(dy, x, mean, rstd, w, has_bias=True)
+    for has_bias in (True, False):
+        got = ffn.layer_norm_backward(dy, x, mean, rstd, w, has_bias=has_bias, need_weight=False)
+        assert torch.equal(got[0], dx) and got[1] is None
+        assert torch.equal(got[2], db) if has_bias else got[2] is None
