@@ -70,9 +70,18 @@ enum class Major { kAny, kK, kMn };
 // tokens: 413, and 499, 481, 639), which a copy of the smaller one can be worth.
 constexpr double kOffSector[3] = {1.0, 1.12, 1.45};
 int64_t sector_pitch(int64_t cols) { return (cols + 15) / 16 * 16; }
-bool off_sector(const Matrix& m) {
-  const int64_t pitch = row_addressable(m) ? row_pitch(m) : row_addressable(transposed(m)) ? row_pitch(transposed(m)) : 0;
-  return !aligned(m.ptr, 32) || pitch % 16 != 0;
+
+// The rows that operand() reads m by where it lies: those of m, or of its
+// transpose, or none (it is copied, to whole sectors).
+enum class Rows { kOwn, kTransposed, kCopied };
+Rows rows_of(const Matrix& m, Major want) {
+  if (want != Major::kMn && row_addressable(m)) return Rows::kOwn;
+  return want != Major::kK && row_addressable(transposed(m)) ? Rows::kTransposed : Rows::kCopied;
+}
+bool off_sector(const Matrix& m, Major want) {
+  const Rows rows = rows_of(m, want);
+  if (rows == Rows::kCopied) return false;
+  return !aligned(m.ptr, 32) || row_pitch(rows == Rows::kOwn ? m : transposed(m)) % 16 != 0;
 }
 // Estimated times in us: a launch and the bytes both ways at 5.5 TB/s; a
 // product at 1.5 PFLOP/s.
@@ -81,16 +90,20 @@ double product_us(int64_t m, int64_t n, int64_t k) {
   return 2.0 * static_cast<double>(m) * static_cast<double>(n) * static_cast<double>(k) / 1.5e9;
 }
 
+// Whether a copy is MN-major: in the order that reads m along its contiguous
+// dimension if `want` leaves the choice.
+bool copied_mn(const Matrix& m, Major want) {
+  return want == Major::kMn || (want == Major::kAny && m.cs != 1 && m.rs == 1);
+}
+
 // m as an operand with m.cols the contraction; `copy`: one whose rows can be
 // read as they are is copied all the same.
 Operand operand(const Matrix& m, Major want, Arena* arena, Copies* copies, bool copy = false) {
   const Matrix t = transposed(m);
-  const bool k_rows = want != Major::kMn && row_addressable(m), mn_rows = want != Major::kK && row_addressable(t);
-  if (!copy && k_rows) return {m.ptr, row_pitch(m), true};
-  if (!copy && mn_rows) return {m.ptr, row_pitch(t), false};
-  // Copied in the order that reads it along its contiguous dimension if the
-  // caller of this function leaves the choice.
-  const bool mn = want == Major::kMn || (want == Major::kAny && m.cs != 1 && m.rs == 1);
+  const Rows rows = copy ? Rows::kCopied : rows_of(m, want);
+  if (rows == Rows::kOwn) return {m.ptr, row_pitch(m), true};
+  if (rows == Rows::kTransposed) return {m.ptr, row_pitch(t), false};
+  const bool mn = copied_mn(m, want);
   const Matrix from = mn ? t : m;
   const int64_t pitch = sector_pitch(from.cols);
   void* to = arena->take(static_cast<size_t>(from.rows) * pitch * kEsz);
@@ -197,15 +210,21 @@ ForwardPlan plan_forward(Product* p, const Matrix& a, const Matrix& b0, const Ma
   bool copy_a = false, copy_b = false;
   p->a[0].k_major = true;
   if (!is_skinny(*p, sm_count)) {
-    const int weights = b1 != nullptr ? 2 : 1;
-    const bool off_a = off_sector(a), off_b = off_sector(b0) || (b1 != nullptr && off_sector(*b1));
-    const double us = product_us(p->m, weights * p->n, p->k);
+    // (the second weight follows the first one's order)
+    const Rows rows = rows_of(b0, Major::kAny);
+    const bool mn = rows == Rows::kTransposed || (rows == Rows::kCopied && copied_mn(b0, Major::kAny));
+    const Major want = mn ? Major::kMn : Major::kK;
+    const bool off_a = off_sector(a, Major::kK);
+    const bool off_b = off_sector(b0, Major::kAny) || (b1 != nullptr && off_sector(*b1, want));
+    double copy_b_us = rows == Rows::kCopied ? 0.0 : copy_us(b0);
+    if (b1 != nullptr && rows_of(*b1, want) != Rows::kCopied) copy_b_us += copy_us(*b1);
+    const double us = product_us(p->m, (b1 != nullptr ? 2 : 1) * p->n, p->k);
     double best = us * kOffSector[off_a + off_b];
     for (int c = 1; c < 4; ++c) {
       const bool ca = (c & 1) != 0, cb = (c & 2) != 0;
       if ((ca && !off_a) || (cb && !off_b)) continue;
       const double t = us * kOffSector[(off_a && !ca) + (off_b && !cb)] + (ca ? copy_us(a) : 0.0) +
-                       (cb ? weights * copy_us(b0) : 0.0);
+                       (cb ? copy_b_us : 0.0);
       if (t < best) best = t, copy_a = ca, copy_b = cb;
     }
   }

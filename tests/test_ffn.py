@@ -127,6 +127,28 @@ def test_workspace_sizes():
     assert lib.glq_layer_norm_backward_workspace_bytes(8, 64) > 0
 
 
+def test_operands_copied_anyway_do_not_weigh_on_the_other():
+    """A with rows that TMA cannot address is copied to whole sectors whatever the plan: B, off its sectors, then
+    decides as beside an A in whole sectors."""
+    lib = native.library()
+
+    def copied(a, a_ld, b, b_ld, m, n, k):
+        size = lib.glq_fused_linear_workspace_bytes(0, a, a_ld, 1, b, 1, b_ld, m, n, k)
+        return size - lib.glq_fused_linear_workspace_bytes(0, P, k, 1, P, 1, k, m, n, k)
+
+    m, n, k = 4096, 2048, 2048
+    assert copied(P, k, P, k + 8, m, n, k) == 0  # (one operand off: not worth a copy)
+    assert copied(P + 2, k + 1, P, k + 8, m, n, k) == m * k * 2
+    assert copied(P, k + 8, P + 2, k + 1, n, m, k) == m * k * 2
+    # The gated pair: an up weight of the other order is copied like that too.
+    def gated_copies(a_ld, u_ks, u_ns):
+        return lib.glq_gated_linear_workspace_bytes(0, P, a_ld, 1, P, 1, k, P, u_ks, u_ns, 8192, 1024, k)
+
+    whole = gated_copies(k, 1, k)
+    assert gated_copies(k + 8, 1, k) == whole
+    assert gated_copies(k + 8, 1032, 1) - whole == 1024 * k * 2
+
+
 @pytest.mark.parametrize("call", [
     lambda a, b: ffn.fused_linear(a, b), lambda a, b: ffn.gated_linear(a, b, b),
     lambda a, b: ffn.fused_linear_backward(a, a, b), lambda a, b: ffn.gated_linear_backward(a, a, b, b, a, a),
