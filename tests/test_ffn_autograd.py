@@ -195,3 +195,24 @@ def test_layer_norm_backward_without_the_weights_gradient(cuda_device):
         got = ffn.layer_norm_backward(dy, x, mean, rstd, w, has_bias=has_bias, need_weight=False)
         assert torch.equal(got[0], dx) and got[1] is None
         assert torch.equal(got[2], db) if has_bias else got[2] is None
+
+
+# ---------------------------------------------------------------- tracing
+
+@pytest.mark.gpu
+def test_custom_ops_trace_ahead_of_time(cuda_device):
+    """Forward and backward graphs traced with symbolic sizes give what the eager calls give."""
+    gen = torch.Generator().manual_seed(8)
+
+    def leaf(*shape):
+        return torch.randn(*shape, generator=gen).to(F16).cuda().requires_grad_()
+
+    a, w, w2, bias, res, scale = leaf(12, 64), leaf(72, 64), leaf(64, 72), leaf(72), leaf(12, 72), leaf(64)
+    ops = torch.ops.gemm_lab
+    tests = ("test_aot_dispatch_dynamic",)
+    for activation in ("silu", None):
+        torch.library.opcheck(ops.fused_linear, (a, w.t(), bias, activation, res), test_utils=tests)
+    torch.library.opcheck(ops.fused_linear, (a, w2, None, None, None, True), test_utils=tests)
+    torch.library.opcheck(ops.gated_linear, (a, w.t(), w2, bias, bias, "gelu"), test_utils=tests)
+    torch.library.opcheck(ops.layer_norm, (a, scale, scale, 1e-5), test_utils=tests)
+    torch.library.opcheck(ops.layer_norm, (a, None, None, 1e-5), test_utils=tests)

@@ -150,3 +150,104 @@ def test_statistics_of_empty_rows():
     torch.full((3,), 7.0, device="cuda")
     y, mean, rstd = ffn.layer_norm(torch.empty((3, 0), dtype=F16, device="cuda"), return_stats=True)
     assert y.shape == (3, 0) and bool(torch.isnan(mean).all()) and bool(torch.isnan(rstd).all())
+
+
+SLOT = 2 * 128 * 256 * 4 + 2 * 8 * 8  # workspace of a dealt run: a pair's partial tile and its flags
+
+
+def runs_of(op, a, bs, n):
+    """Dealt runs of a forward call on aligned operands in whole sectors: what its workspace is for."""
+    m, k = a.shape
+    args = [int(a.dtype == BF16), a.data_ptr(), k, 1]
+    for b in bs:
+        args += [b.data_ptr(), b.stride(0), b.stride(1)]
+    size = getattr(native.library(), f"glq_{op}_workspace_bytes")(*args, m, n, k)
+    runs = size // SLOT
+    assert size == (runs * SLOT + 255) // 256 * 256
+    return runs
+
+
+@pytest.mark.parametrize("m,n,k,act,order,dtype", [
+    (500, 10240, 8192, "gelu", "nk", BF16),  # 80 tiles: 74 whole, the blocks of 6 dealt
+    (700, 6500, 8192, "silu", "nk", F16),    # rows off 16 bytes: stored element by element
+    (300, 9808, 8192, None, "kn", BF16),
+])
+def test_dealt_remainder_of_a_linear_layer(m, n, k, act, order, dtype):
+    """Whole tiles first, then runs joined through the workspace, with bias, activation, residual and kept z."""
+    gen = torch.Generator().manual_seed(n)
+    a, bias, res = make(gen, dtype, m, k), make(gen, dtype, n), make(gen, dtype, m, n)
+    b = make(gen, dtype, n, k, scale=k ** -0.5).t() if order == "nk" else make(gen, dtype, k, n, scale=k ** -0.5)
+    assert runs_of("fused_linear", a, (b,), n) > 0
+    y, z = ffn.fused_linear(a, b, bias, act, res, return_preact=True)
+    wy, wz, ey, ez = ref.linear(d(a), d(b), d(bias), act, d(res), dtype)
+    ref.within(y, wy, ey, "y")
+    ref.within(z, wz, ez, "z")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = ffn.fused_linear(a, b, bias, act, res)
+    for _ in range(3):
+        again.zero_()
+        graph.replay()
+        assert torch.equal(again, y)
+
+
+@pytest.mark.parametrize("m,n,k,dtype", [
+    (500, 8192, 11008, BF16),  # 128 tiles: 74 whole, 54 dealt to every pair
+    (300, 5004, 8192, F16),    # few pairs have a run; rows off 16 bytes
+])
+def test_dealt_remainder_of_a_gated_pair(m, n, k, dtype):
+    gen = torch.Generator().manual_seed(n)
+    a, bias_g, bias_u = make(gen, dtype, m, k), make(gen, dtype, n), make(gen, dtype, n)
+    bg, bu = (make(gen, dtype, n, k, scale=k ** -0.5).t() for _ in range(2))
+    assert runs_of("gated_linear", a, (bg, bu), n) > 0
+    h, g, u = ffn.gated_linear(a, bg, bu, bias_g, bias_u, "gelu_tanh", return_preact=True)
+    wh, wg, wu, eh, eg, eu = ref.gated(d(a), d(bg), d(bu), d(bias_g), d(bias_u), "gelu_tanh", dtype)
+    for got, want, bound in ((h, wh, eh), (g, wg, eg), (u, wu, eu)):
+        ref.within(got, want, bound, "gated")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = ffn.gated_linear(a, bg, bu, bias_g, bias_u, "gelu_tanh")
+    for _ in range(3):
+        again.zero_()
+        graph.replay()
+        assert torch.equal(again, h)
+
+
+@pytest.mark.parametrize("m", [20, 300])
+def test_non_finite_gradients_stay_in_their_rows(m):
+    gen = torch.Generator().manual_seed(3)
+    n, k = 136, 200
+    a, z, u, dy = make(gen, F16, m, k), make(gen, F16, m, n), make(gen, F16, m, n), make(gen, F16, m, n)
+    b, b2 = (make(gen, F16, n, k, scale=k ** -0.5).t() for _ in range(2))
+    _, mean, rstd = ffn.layer_norm(z, return_stats=True)
+
+    def input_gradients(dy):
+        return [ffn.fused_linear_backward(dy, a, b, z, "silu")[0], ffn.gated_linear_backward(dy, a, b, b2, z, u, "gelu")[0],
+                ffn.layer_norm_backward(dy, z, mean, rstd)[0]]
+
+    clean = input_gradients(dy)
+    dy[7, 3], dy[11, 5] = float("nan"), float("inf")
+    keep = [i for i in range(m) if i not in (7, 11)]
+    for got, was in zip(input_gradients(dy), clean):
+        assert bool(torch.isnan(got[7]).all()) and not bool(torch.isfinite(got[11]).all())
+        assert torch.equal(got[keep], was[keep])
+    # A column's sum sees what is in its column alone.
+    dbias = ffn.fused_linear_backward(dy, a, b, z, "silu", has_bias=True, need_a=False, need_b=False)[2]
+    assert [i for i in range(n) if not math.isfinite(float(dbias[i]))] == [3, 5]
+
+
+@pytest.mark.parametrize("n", [264, 1001])
+def test_layer_norm_near_the_largest_float16(n):
+    gen = torch.Generator().manual_seed(n)
+    x = (torch.randint(0, 2, (6, n), generator=gen) * 2.0 - 1.0).mul(65504.0).to(F16).cuda()
+    x[1] = 65504.0
+    x[2] = 2.0 ** -24
+    w, b, dy = make(gen, F16, n, scale=0.2) + 1, make(gen, F16, n), make(gen, F16, 6, n)
+    y, mean, rstd = ffn.layer_norm(x, w, b, 1e-5, return_stats=True)
+    wy, wm, wr, ey, em, er = ref.layer_norm(d(x), d(w), d(b), 1e-5, F16)
+    ref.within(mean, wm, em, "mean")
+    ref.within(rstd, wr, er, "rstd")
+    ref.within(y, wy, ey, "y")
+    got = ffn.layer_norm_backward(dy, x, mean, rstd, w, has_bias=True)
+    for g, (v, bound) in zip(got, ref.layer_norm_backward(d(dy), d(x), d(mean), d(rstd), d(w), F16)):
+        ref.within(g, v, bound, "gradient")
