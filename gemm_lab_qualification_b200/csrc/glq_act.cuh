@@ -18,7 +18,6 @@ struct Elem16;
 template <>
 struct Elem16<__half> {
   static constexpr int kFormat = 0;  // tcgen05 kind::f16 operand format
-  using Pair = __half2;
   __device__ static float to_f(__half v) { return __half2float(v); }
   __device__ static __half from_f(float v) { return __float2half_rn(v); }
   __device__ static float2 to_f2(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
@@ -31,7 +30,6 @@ struct Elem16<__half> {
 template <>
 struct Elem16<__nv_bfloat16> {
   static constexpr int kFormat = 1;
-  using Pair = __nv_bfloat162;
   __device__ static float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
   __device__ static __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
   __device__ static float2 to_f2(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }

@@ -87,4 +87,8 @@ cudaError_t skinny_prepare_device();
 bool encode_tile_map(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t cols, int64_t pitch,
                      uint32_t box_rows, uint32_t box_cols = 64);
 
+// The map of an operand with `rows` output rows and contraction `k`: boxes of
+// box_rows rows x 64 K, or 64 rows x 64 K when MN-major.
+bool operand_map(CUtensorMap* map, int dtype, const Operand& o, int64_t rows, int64_t k, uint32_t box_rows);
+
 }  // namespace glq

@@ -694,7 +694,6 @@ int glq_layer_norm(int dtype, const void* X, int64_t x_row_stride, const void* w
   a.rows = M;
   a.cols = static_cast<int>(N);
   a.eps = static_cast<float>(eps);
-  a.err = err;
   return glq::status_of(glq::launch_norm(dtype, a, sm_count, flags, static_cast<cudaStream_t>(stream)));
 }
 

@@ -3,6 +3,7 @@
 // surface.
 #pragma once
 
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <cstddef>
@@ -240,6 +241,9 @@ cudaError_t launch_repack(const void* src, int64_t rows, int64_t cols, int64_t r
 // two-CTAs-per-SM split with stages == kPairStagesKps2).
 cudaError_t launch_tc(const Problem& p, int split, int tile_t, int tile_n, int stages, int kps, int w_mn,
                       const Gather* gather, unsigned int* err, cudaStream_t s);
+
+// The driver's cuTensorMapEncodeTiled, looked up once (null: it has none).
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
 // Per-device one-time set-up of the tcgen05 kernels (shared memory opt-in).
 cudaError_t tc_prepare_device();

@@ -46,7 +46,6 @@
 // Every wait is bounded; an expired one raises a bit in the device error word
 // and the kernel returns.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <atomic>
@@ -763,13 +762,6 @@ unsigned long long next_epoch() {
 
 bool aligned_rows(const void* p, int64_t ld) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * 2) % 16 == 0;
-}
-
-// The map of an operand with `rows` output rows and contraction `k`: boxes of
-// box_rows rows x 64 K, or 64 rows x 64 K when MN-major.
-bool operand_map(CUtensorMap* map, int dtype, const Operand& o, int64_t rows, int64_t k, uint32_t box_rows) {
-  return o.k_major ? encode_tile_map(map, dtype, o.base, rows, k, o.pitch, box_rows)
-                   : encode_tile_map(map, dtype, o.base, k, rows, o.pitch, kBK);
 }
 
 template <typename T, bool GATED, bool SPLIT>

@@ -25,7 +25,6 @@ struct NormArgs {
   long long rows;
   int cols;
   float eps;
-  unsigned int* err;
   int align, align_w;  // bytes that rows, weight and bias start at multiples of
   int vec;             // rows of whole 16-byte vectors
 };

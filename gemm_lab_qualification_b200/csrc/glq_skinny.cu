@@ -406,11 +406,6 @@ __global__ void __launch_bounds__(kThreads, SkinnyConfig<BT>::kPerSm)
   }
 }
 
-bool operand_map(CUtensorMap* map, int dtype, const Operand& o, int64_t rows, int64_t k, uint32_t box_rows) {
-  return o.k_major ? encode_tile_map(map, dtype, o.base, rows, k, o.pitch, box_rows)
-                   : encode_tile_map(map, dtype, o.base, k, rows, o.pitch, kBK);
-}
-
 template <typename T, int BT, bool W_MN, bool GATED>
 cudaError_t launch_typed(const Product& p, int sm_count, unsigned int* err, cudaStream_t s) {
   using Cfg = SkinnyConfig<BT>;

@@ -51,12 +51,10 @@
 // (kernels.py:73-129, 191-249, 324-393), which compute the same sums with
 // B = [K, N] operands on sm_80+ mma.sync.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "glq_internal.h"
 #include "glq_ptx.cuh"
@@ -1095,27 +1093,11 @@ __global__ void __launch_bounds__(kThreads, RAW != 0 ? 2 : 1)
 
 // ------------------------------------------------------------------ host
 
-PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-std::once_flag g_encode_once;
-
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  std::call_once(g_encode_once, [] {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault,
-                                         &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess) {
-      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-  });
-  return g_encode;
-}
-
 // 2-D map of a row-major matrix rows x cols (cols contiguous) with a row
 // pitch in bytes; box box_rows x box_cols, 128-byte swizzle, OOB zero fill.
 bool encode_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t cols, int64_t rows,
                int64_t row_pitch_bytes, uint32_t box_cols, uint32_t box_rows) {
-  PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (encode == nullptr) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_pitch_bytes)};
@@ -1134,7 +1116,7 @@ bool encode_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int
 // two 2-D boxes of 64 x box_rows at consecutive K blocks would give.
 bool encode_kblocks_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t k, int64_t rows,
                        int64_t row_pitch_bytes, uint32_t box_rows) {
-  PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (encode == nullptr || k % kTileK != 0) return false;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(kTileK), static_cast<cuuint64_t>(rows),
                               static_cast<cuuint64_t>(k / kTileK)};
@@ -1154,7 +1136,7 @@ bool encode_kblocks_3d(CUtensorMap* map, CUtensorMapDataType type, const void* b
 // what box_blocks 2-D boxes of 64 x box_k would write.
 bool encode_mn_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t n, int64_t k,
                   int64_t row_pitch_bytes, uint32_t box_k, uint32_t box_blocks) {
-  PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (encode == nullptr || n % 64 != 0) return false;
   const cuuint64_t dims[3] = {64u, static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(n / 64)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_pitch_bytes), 128u};
@@ -1176,7 +1158,7 @@ bool encode_mn_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, 
 bool encode_raw(CUtensorMap* maps, CUtensorMapDataType type, const void* base, int64_t rows, int64_t k,
                 int64_t pitch, int tile_rows, RawClasses* rc) {
   if (!raw_classes(base, rows, k, pitch, rc)) return false;
-  PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (encode == nullptr) return false;
   const uintptr_t b = reinterpret_cast<uintptr_t>(base);
   const uintptr_t b_aligned = b & ~static_cast<uintptr_t>(15);

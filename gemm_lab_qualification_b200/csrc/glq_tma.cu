@@ -1,4 +1,5 @@
-// glq_tma.cu -- tensor maps of the feed-forward operators' products.
+// glq_tma.cu -- the driver's tensor-map encoder, and the maps of the
+// feed-forward operators' products.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -6,6 +7,7 @@
 #include <mutex>
 
 #include "glq_ffn.h"
+#include "glq_internal.h"
 
 namespace glq {
 namespace {
@@ -13,7 +15,9 @@ namespace {
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+}  // namespace
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
@@ -25,11 +29,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return g_encode;
 }
 
-}  // namespace
-
 bool encode_tile_map(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t cols, int64_t pitch,
                      uint32_t box_rows, uint32_t box_cols) {
-  PFN_cuTensorMapEncodeTiled_v12000 encode = encoder();
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (encode == nullptr) return false;
   const CUtensorMapDataType type =
       dtype == GLQ_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -40,6 +42,11 @@ bool encode_tile_map(CUtensorMap* map, int dtype, const void* base, int64_t rows
   return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool operand_map(CUtensorMap* map, int dtype, const Operand& o, int64_t rows, int64_t k, uint32_t box_rows) {
+  return o.k_major ? encode_tile_map(map, dtype, o.base, rows, k, o.pitch, box_rows)
+                   : encode_tile_map(map, dtype, o.base, k, rows, o.pitch, 64);
 }
 
 }  // namespace glq
