@@ -310,6 +310,15 @@ __device__ __forceinline__ uint4 ld_smem_v4(uint32_t at) {
 // per SM to hide behind), and arithmetic is paired.  VEC: rows of whole
 // 16-byte vectors; other rows are held in pairs of columns (Columns).
 
+// sum / n with inv = 1 / n rounded: the product and its remainder's share, so
+// that the mean of a constant row is its value (sum * inv can be one bit off,
+// which rstd magnifies).  A division here costs 2 % at 16384 x 8192.
+__device__ __forceinline__ float quotient(float sum, float n, float inv) {
+  const float q = sum * inv;
+  const float exact = fmaf(fmaf(-q, n, sum), inv, q);
+  return fabsf(q) <= 3.402823466e38f ? exact : q;  // (infinity has no remainder)
+}
+
 constexpr int kNormThreads = 256;
 
 template <typename T, int G, int V, bool VEC>
@@ -355,8 +364,7 @@ __global__ void __launch_bounds__(G < kNormThreads ? kNormThreads : G, G < 512 ?
     if (r + step < a.rows) request(r + step);
     float sum[1] = {halves(acc).x + halves(acc).y};
     row_sum<G>(sum, my_red, phase, group);
-    // (a division: the rounding of 1 / cols, times rstd, shows in constant rows)
-    const float mean = sum[0] / static_cast<float>(cols);
+    const float mean = quotient(sum[0], static_cast<float>(cols), inv);
     const Two minus_mean = two(-mean, -mean);
     acc = 0;
 #pragma unroll
@@ -440,7 +448,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a) {
       for (int i = 0; i < 8; ++i) sum[0] += v[i];
     }
     row_sum<1024>(sum, red, phase, 0);
-    const float mean = sum[0] / static_cast<float>(a.cols);
+    const float mean = quotient(sum[0], static_cast<float>(a.cols), inv);
     for (int c = threadIdx.x * 8; c < a.cols; c += 1024 * 8) {
       load8(x + c, a.align, a.cols - c, v);
       for (int i = 0; i < 8; ++i) {

@@ -144,6 +144,15 @@ def test_layer_norm_of_constant_rows(n, dtype):
     assert float((rstd.double() * math.sqrt(1e-5) - 1).abs().max()) <= 2.0 ** -21
 
 
+@pytest.mark.parametrize("n", [264, 4095, 20001])
+def test_statistics_of_infinite_rows(n):
+    x = torch.zeros((3, n), dtype=BF16, device="cuda")
+    x[0, 5], x[1, 6], x[2, 7] = math.inf, -math.inf, math.nan
+    y, mean, _ = ffn.layer_norm(x, return_stats=True)
+    assert float(mean[0]) == math.inf and float(mean[1]) == -math.inf and math.isnan(float(mean[2]))
+    assert not bool(torch.isfinite(y).any())
+
+
 def test_statistics_of_empty_rows():
     """The mean of no values is 0 / 0, and so is their variance: not what the memory held before."""
     torch.full((3,), 7.0, device="cuda")  # the block that the statistics will take
