@@ -13,6 +13,7 @@ operands' device:
 * ``layer_norm`` -- row normalisation with weight and bias;
 * ``feed_forward`` -- the pre-norm block that they make up.
 
+Rows, columns and contraction of the products go up to 65535 * 64.
 ``activation`` is None, "silu", "gelu" (exact), "gelu_tanh" or "relu".
 
 Called on tensors that require gradients, they are differentiable: the call
@@ -21,8 +22,9 @@ tracing), which keeps what its backward pass reads.  The ``*_backward``
 functions are those passes for callers that run their own.  Gradients have
 the inputs' 16-bit type; every sum is FP32 with one rounding, except that the
 gradient of the pre-activations is rounded to 16 bits before the products that
-read it.  The backward passes themselves are not differentiable,
-and forward-mode tangents (``torch.autograd.forward_ad``) are refused.
+read it (in float16 it overflows beyond 65504).  The backward passes
+themselves are not differentiable, and forward-mode tangents
+(``torch.autograd.forward_ad``) are refused.
 
 The ``*_into`` forms write in place and raise the version of what they wrote,
 as torch's own operations do: a pending backward pass that saved the tensor

@@ -112,7 +112,9 @@ enum glq_flags {
   /* The weight operand B is not written by the kernel that precedes this call
    * in the stream (true for inference weights).  The kernel then starts
    * streaming B before the dependency wait, overlapping the predecessor's
-   * tail.  Only A, bias and Y wait for the predecessor. */
+   * tail.  Only A, bias and Y wait for the predecessor.  (The feed-forward
+   * operators' kernel for up to 192 tokens heeds it; those for many tokens and
+   * for one token with K-contiguous weights load after the wait.) */
   GLQ_FLAG_STATIC_WEIGHTS = 1u << 1
 };
 
@@ -363,6 +365,7 @@ enum glq_activation {
  *   - Optional pointers may be NULL; an output that is NULL is not computed.
  *   - Outputs must not overlap inputs or each other, except that Y of
  *     glq_fused_linear may be its residual (same address and row stride).
+ *   - M, N and K of the products are at most 65535 * 64 (GLQ_ERR_SHAPE).
  *   - Every sum has a fixed order, so a call gives the same bits every time;
  *     the order depends on the sizes and on which outputs are asked for.
  *   - flags: enum glq_flags.
