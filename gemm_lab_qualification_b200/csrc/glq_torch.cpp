@@ -413,8 +413,8 @@ std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm(const at::Tensor& x
 
 std::tuple<int, at::Tensor, OptTensor, OptTensor> layer_norm_backward(const at::Tensor& grad, const at::Tensor& x,
                                                                       const at::Tensor& mean, const at::Tensor& rstd,
-                                                                      const OptTensor& weight, bool has_bias, bool need_weight,
-                                                                      int64_t flags) {
+                                                                      const OptTensor& weight, bool has_bias,
+                                                                      bool need_weight, int64_t flags) {
   check_no_tangent("layer_norm_backward", grad, x, mean, rstd, weight);
   check_norm(x, "layer_norm_backward");
   const c10::cuda::CUDAGuard guard(x.device());
